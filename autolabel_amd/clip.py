@@ -1,0 +1,85 @@
+"""The global norm of the gradients, and their clipping by it (csrc/clip.hip).
+
+Not part of the reference's loop (autolabel/trainer.py:39-49 steps its optimizers on unclipped gradients); here it stands between the backward
+pass and the optimizer: ``TrainEngine(max_grad_norm=...)`` / ``Trainer(max_grad_norm=...)`` / ``scripts/train.py --max-grad-norm``, or by hand:
+
+    norm = clip.clip_grad_norm_([p.grad for p in model.parameters() if p.grad is not None], 1.0)
+
+One launch for the squares and one for the scaling per 120 tensors, whatever their sizes and types; the norm stays on the device.
+"""
+import contextlib
+import ctypes as C
+import math
+
+import torch
+
+from . import hip as H
+
+TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _dense(t):
+    """True when the elements of t fill one run of memory without holes or overlaps (in any order of its axes)."""
+    if t.is_contiguous():
+        return True
+    order = sorted((d for d in range(t.dim()) if t.shape[d] > 1), key=t.stride)
+    step = 1
+    for d in order:
+        if t.stride(d) != step:
+            return False
+        step *= t.shape[d]
+    return True
+
+
+def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
+    grads = [grads] if torch.is_tensor(grads) else list(grads)
+    if not grads:
+        raise ValueError(f'{name}: an empty list of tensors')
+    dev = getattr(grads[0], 'device', None)
+    for i, t in enumerate(grads):
+        if not torch.is_tensor(t) or t.dtype not in TYPES or t.layout != torch.strided:
+            raise ValueError(f'{name}: tensor {i} must be a dense fp16, bf16 or fp32 tensor')
+        if not _dense(t):
+            raise ValueError(f'{name}: tensor {i} with shape {tuple(t.shape)} and strides {t.stride()} does not fill one run of memory')
+        if t.device != dev:
+            raise ValueError(f'{name}: tensors on different devices: {dev} and {t.device}')
+    if out is not None:
+        out = [out] if torch.is_tensor(out) else list(out)
+        if len(out) != len(grads):
+            raise ValueError(f'{name}: {len(grads)} tensors, {len(out)} outputs')
+        for i, (t, o) in enumerate(zip(grads, out)):
+            if o.dtype != t.dtype or o.shape != t.shape or o.device != dev or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous())):
+                raise ValueError(f'{name}: output {i} must have the type, shape, strides and device of its tensor')
+    for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32)):
+        if w is not None and (not torch.is_tensor(w) or w.dtype != dt or w.numel() < 1 or w.device != dev):
+            raise ValueError(f'{name}: {what} must be a device tensor of {dt} beside the gradients')
+    if not dev.type == 'cuda':
+        raise ValueError(f'{name}: autolabel_amd.clip has no CPU path: needs device tensors')
+    n = len(grads)
+    with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws = torch.empty(int(H.lib().aln_grad_clip_ws_bytes(n)), dtype=torch.uint8, device=dev)
+        pointers = C.c_void_p * n
+        H.call('aln_grad_clip', n, pointers(*[t.data_ptr() for t in grads]), pointers(*[t.data_ptr() for t in out]) if out is not None else None,
+               (C.c_int64 * n)(*[t.numel() for t in grads]), (C.c_int32 * n)(*[TYPES[t.dtype] for t in grads]), max_norm, int(apply),
+               H.C.c_void_p(loss_scale.data_ptr()) if loss_scale is not None else None, H.C.c_void_p(norm.data_ptr()),
+               H.C.c_void_p(found_inf.data_ptr()) if found_inf is not None else None, H.C.c_void_p(ws.data_ptr()), ws.numel(), H.stream())
+    return norm
+
+
+def grad_norm(grads, loss_scale=None, found_inf=None):
+    """sqrt of the sum of all squares of the tensors ``grads``, over ``loss_scale`` -> fp32 scalar on the device (squares and sums in fp64;
+    the same bits on every call).  ``found_inf`` (int32, device) is set to 1 when the norm is not finite."""
+    return _launch('grad_norm', grads, 0.0, False, None, loss_scale, found_inf)
+
+
+def clip_grad_norm_(grads, max_norm, out=None, loss_scale=None, found_inf=None):
+    """Scale the tensors ``grads`` by min(1, max_norm / (norm + 1e-6)), in place or into ``out``, and return their ``grad_norm``.
+
+    The tensors may differ in type (fp16, bf16, fp32) and size; no two may share memory.  Gradients that a loss scaler has multiplied keep
+    its factor: ``loss_scale`` (fp32, device) only divides the norm.  A norm that is not finite scales nothing (``out`` is then a copy) and
+    sets ``found_inf``: the caller skips that step."""
+    max_norm = float(max_norm)
+    if math.isnan(max_norm) or max_norm < 0:
+        raise ValueError(f'clip_grad_norm_: max_norm = {max_norm}')
+    return _launch('clip_grad_norm_', grads, max_norm, True, out, loss_scale, found_inf)

@@ -1,0 +1,473 @@
+// Products in 8-bit floating point with one power-of-two scale per block of 128 along the contracted axis, and the quantisers that feed them
+// (no counterpart in the reference: its semantic heads, autolabel/models.py:117-136, run in fp16 through tinycudann).
+//
+// A row x[0, K) is cut into blocks of 128; a block is held as q (e4m3 or e5m2) and ONE exponent e, x ~ q 2^e:
+//     e = the smallest e >= -126 with max |x| 2^-e <= 448 (e4m3) or 57344 (e5m2);   0 for a block of zeros
+//     q = x 2^-e rounded to the nearest 8-bit value, ties to even
+// Both types' largest value is 1.75 2^EMAX (EMAX = 8, 15), so e = exponent(max) - EMAX, plus one where max's mantissa is above 1.75: nothing is
+// clipped, and since 2^-e x is exact, q is one rounding of x whatever the order of the arithmetic.  A power of two costs a floating type no
+// precision against an fp32 scale (only the top fraction of a binade of range), and it is what v_mfma_scale_f32_32x32x64_f8f6f4 takes as an
+// operand: y = sum_b 2^(ex_b + ew_b) sum_{k in b} qx qw costs no instruction beside the matrix instructions.
+// That instruction accumulates in fp32, but aligns the 64 products of a step to the largest of them and drops what lies 13 binades below it
+// (measured; the older v_mfma_f32_32x32x16_fp8_fp8 does the same): 1.3e-5 of the result for Gaussian operands, 7e-5 for values spread over 12
+// binades.  Under the half step of a 16-bit result (4.9e-4, 3.9e-3), far above that of an fp32 one: products with an fp32 result turn the 8-bit
+// values back into bf16, which holds q 2^e exactly, and use the bf16 instruction (5e-8, at half the rate).
+// A block that holds an infinity or a NaN is NaN throughout (its row of the product would be non-finite in every column anyway).
+//
+// Layout: q [rows, ldq] bytes, columns [K, 128 ceil(K / 128)) zero; scale [rows, lds] bytes e + 127, lds a multiple of 4, so that the four
+// scales of 512 columns are one aligned 4-byte word.
+#include "common.h"
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
+
+enum { F8_E4M3 = 0, F8_E5M2 = 1 };                       // also the format codes of the matrix instruction
+enum { FT_F16 = 0, FT_BF16 = 1, FT_F32 = 2 };
+static inline int64_t ceil128(int64_t n) { return (n + 127) / 128 * 128; }
+
+// ---------------------------------------------------------------------------------------------------------- block arithmetic
+template <int CTRL> __device__ inline uint32_t dpp_umax(uint32_t v) {
+  const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false);
+  return v > o ? v : o;
+}
+// the maximum over the 16 lanes of a row of the wave, in every one of them
+__device__ inline uint32_t umax16(uint32_t v) {
+  v = dpp_umax<0xB1>(v);    // quad_perm 1,0,3,2
+  v = dpp_umax<0x4E>(v);    // quad_perm 2,3,0,1
+  v = dpp_umax<0x141>(v);   // row_half_mirror
+  return dpp_umax<0x140>(v);  // row_mirror
+}
+
+// e of a block from the bits of max |x| as fp32 (NaN and infinity compare above every finite value), and the factor 2^-e (NaN for such a block)
+template <int FMT> __device__ inline int block_exp(uint32_t amax_bits, float& factor) {
+  constexpr int EMAX = FMT == F8_E4M3 ? 8 : 15;
+  int e = (int)(amax_bits >> 23) - 127 - EMAX + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  if (e < -126) e = -126;
+  if (amax_bits == 0) e = 0;
+  factor = __uint_as_float(amax_bits >= 0x7f800000u ? 0x7fc00000u : (uint32_t)(127 - e) << 23);
+  return e;
+}
+
+template <int FMT> __device__ inline uint32_t pack4(float a, float b, float c, float d) {
+  int w = 0;
+  if constexpr (FMT == F8_E4M3) { w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, w, false); w = __builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true); }
+  else { w = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, w, false); w = __builtin_amdgcn_cvt_pk_bf8_f32(c, d, w, true); }
+  return (uint32_t)w;
+}
+
+// Eight consecutive values of a row as they are stored, the bits of their largest |x| as fp32, and their fp32 values.  Loads go through
+// memcpy: a row of an odd number of columns is only aligned to its element.
+template <int T> struct Eight;
+template <> struct Eight<FT_F16> {
+  u16x8 v;
+  __device__ void load(const void* p, int64_t at, int n) {
+    const uint16_t* s = (const uint16_t*)p + at;
+    if (n >= 8) __builtin_memcpy(&v, s, 16);
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? s[j] : (uint16_t)0;
+    }
+  }
+  __device__ uint32_t amax() const {
+    const u16x8 a = v & (uint16_t)0x7fff;
+    uint16_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = a[j] > m ? a[j] : m;
+    return __float_as_uint((float)__builtin_bit_cast(h16, m));
+  }
+  __device__ float get(int j) const { return (float)__builtin_bit_cast(h16, (uint16_t)v[j]); }
+};
+template <> struct Eight<FT_BF16> {
+  u16x8 v;
+  __device__ void load(const void* p, int64_t at, int n) {
+    const uint16_t* s = (const uint16_t*)p + at;
+    if (n >= 8) __builtin_memcpy(&v, s, 16);
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? s[j] : (uint16_t)0;
+    }
+  }
+  __device__ uint32_t amax() const {
+    const u16x8 a = v & (uint16_t)0x7fff;
+    uint16_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m = a[j] > m ? a[j] : m;
+    return (uint32_t)m << 16;
+  }
+  __device__ float get(int j) const { return __uint_as_float((uint32_t)v[j] << 16); }
+};
+template <> struct Eight<FT_F32> {
+  float v[8];
+  __device__ void load(const void* p, int64_t at, int n) {
+    const float* s = (const float*)p + at;
+    if (n >= 8) __builtin_memcpy(v, s, 32);
+    else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < n ? s[j] : 0.f;
+    }
+  }
+  __device__ uint32_t amax() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) { const uint32_t a = __float_as_uint(v[j]) & 0x7fffffffu; m = a > m ? a : m; }
+    return m;
+  }
+  __device__ float get(int j) const { return v[j]; }
+};
+
+template <int T, int FMT> __device__ inline uint2 quant8(const Eight<T>& x, float f) {
+  return make_uint2(pack4<FMT>(x.get(0) * f, x.get(1) * f, x.get(2) * f, x.get(3) * f), pack4<FMT>(x.get(4) * f, x.get(5) * f, x.get(6) * f, x.get(7) * f));
+}
+
+// ------------------------------------------------------------------------------------------------------------ quantisers
+// Rows: 16 lanes hold a block (8 values each), its maximum goes round them with four DPP steps; one read of x, one write of q.
+template <int T, int FMT>
+__global__ __launch_bounds__(256) void k_fp8_quant(const void* __restrict__ x, int64_t ldx, int64_t M, int K, int nb, uint8_t* __restrict__ q,
+                                                   int64_t ldq, uint8_t* __restrict__ scale, int64_t lds) {
+  const int sub = threadIdx.x & 15;
+  for (int64_t i = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 4; i < M * nb; i += (int64_t)gridDim.x * 16) {
+    const int64_t row = i / nb;
+    const int b = (int)(i - row * nb), k = b * 128 + sub * 8;
+    Eight<T> v;
+    v.load(x, row * ldx + k, K - k);
+    float f;
+    const int e = block_exp<FMT>(umax16(v.amax()), f);
+    *(uint2*)(q + row * ldq + k) = quant8<T, FMT>(v, f);
+    if (sub == 0) scale[row * lds + b] = (uint8_t)(e + 127);
+    else if (sub < 4 && b == nb - 1 && nb + sub - 1 < (nb + 3) / 4 * 4) scale[row * lds + nb + sub - 1] = 127;   // the rest of the last word
+  }
+}
+
+// Columns: q of x^T with blocks of 128 along the rows of x.  A block of threads turns a tile of 128 rows x 64 columns round: a thread reads
+// eight columns of four rows, the maxima of a column meet through three shuffles and LDS, the 8-bit values cross in LDS and leave as whole
+// 128-byte lines.
+template <int T, int FMT>
+__global__ __launch_bounds__(256) void k_fp8_quant_t(const void* __restrict__ x, int64_t ldx, int64_t M, int C, int nb, uint8_t* __restrict__ q,
+                                                     int64_t ldq, uint8_t* __restrict__ scale, int64_t lds) {
+  __shared__ uint32_t amax[4][64];
+  __shared__ __attribute__((aligned(16))) uint8_t tile[64][144];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c8 = (tid & 7) * 8, r0 = tid >> 3;   // rows r0 + 32 i
+  const int nct = (C + 63) / 64;
+  const int64_t b = blockIdx.x / nct;
+  const int c0 = (int)(blockIdx.x % nct) * 64;
+  Eight<T> v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t row = b * 128 + r0 + 32 * i;
+    v[i].load(x, row * ldx + c0 + c8, row < M ? C - c0 - c8 : 0);
+  }
+  uint32_t m[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    m[j] = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { const uint32_t a = __float_as_uint(v[i].get(j)) & 0x7fffffffu; m[j] = a > m[j] ? a : m[j]; }
+#pragma unroll
+    for (int o = 8; o < 64; o <<= 1) { const uint32_t a = (uint32_t)__shfl_xor((int)m[j], o); m[j] = a > m[j] ? a : m[j]; }
+  }
+  if (lane < 8) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) amax[wave][c8 + j] = m[j];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    uint32_t a = amax[0][c8 + j];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) a = amax[w][c8 + j] > a ? amax[w][c8 + j] : a;
+    float f;
+    const int e = block_exp<FMT>(a, f);
+    const uint32_t p = pack4<FMT>(v[0].get(j) * f, v[1].get(j) * f, v[2].get(j) * f, v[3].get(j) * f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) tile[c8 + j][r0 + 32 * i] = (uint8_t)(p >> (8 * i));
+    if (tid < 8 && c0 + c8 + j < C) {
+      scale[(c0 + c8 + j) * lds + b] = (uint8_t)(e + 127);
+      if (b == nb - 1) for (int k = nb; k < (nb + 3) / 4 * 4; ++k) scale[(c0 + c8 + j) * lds + k] = 127;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int c = (tid >> 3) + 32 * i;
+    if (c0 + c < C) *(uint4*)(q + (c0 + c) * ldq + b * 128 + (tid & 7) * 16) = *(const uint4*)&tile[c][(tid & 7) * 16];
+  }
+}
+
+// -------------------------------------------------------------------------------------------------------------- products
+template <int FA, int FB> __device__ inline f32x16 mfma8(i32x8 a, i32x8 b, f32x16 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, 0, sa, 0, sb);
+}
+
+// two 8-bit values (the upper two of the word with HI) times a power of two, exact in bf16
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
+template <int FMT, bool HI> __device__ inline b16x2 widen2(uint32_t w, float s) {
+  if constexpr (FMT == F8_E4M3) return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, HI);
+  else return __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8(w, s, HI);
+}
+template <int FMT> __device__ inline b16x8 widen8(uint32_t w0, uint32_t w1, float s) {
+  const b16x2 a = widen2<FMT, false>(w0, s), b = widen2<FMT, true>(w0, s), c = widen2<FMT, false>(w1, s), d = widen2<FMT, true>(w1, s);
+  return (b16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+
+struct Fp8Out { void* y; int64_t ldy; int type, relu; };   // type: FT_*
+
+// One wave's 32 x 64 block of the result.  The accumulators hold D[n][m]: lane = row m of y (lane % 32), register r = column
+// 8 (r / 4) + 4 (lane / 32) + r % 4 -- stores from there would touch 32 rows per instruction with 8 bytes each, so the block, already rounded
+// to its type, goes round through LDS (`buf`, the wave's own 32 x 272 bytes) and leaves row by row, 16 bytes a lane.
+__device__ inline void store_block(const Fp8Out& o, const f32x16& c0, const f32x16& c1, uint8_t* buf, int64_t m0, int64_t M, int n0, int N, int lane) {
+  const int r = lane & 31, h = lane >> 5, es = o.type == FT_F32 ? 4 : 2, pitch = 64 * es + 16;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { v[j] = s ? c1[4 * g + j] : c0[4 * g + j]; if (o.relu) v[j] = v[j] < 0.f ? 0.f : v[j]; }   // (a NaN stays)
+      const int col = 32 * s + 8 * g + 4 * h;
+      if (o.type == FT_F32) *(f32x4*)(buf + r * pitch + 4 * col) = (f32x4){v[0], v[1], v[2], v[3]};
+      else if (o.type == FT_F16) *(h16x4*)(buf + r * pitch + 2 * col) = (h16x4){(h16)v[0], (h16)v[1], (h16)v[2], (h16)v[3]};
+      else {
+        typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
+        *(b16x4*)(buf + r * pitch + 2 * col) = (b16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+      }
+    }
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  const int lpr = 4 * es, per = 16 / es;            // lanes per row of 64 values, values per lane
+  for (int i = lane; i < 32 * lpr; i += 64) {
+    const int row = i / lpr, c = (i % lpr) * per;
+    const int64_t m = m0 + row;
+    if (m >= M || n0 + c >= N) continue;
+    const uint4 w = *(const uint4*)(buf + row * pitch + c * es);
+    uint8_t* p = (uint8_t*)o.y + (m * o.ldy + n0 + c) * es;
+    if (n0 + c + per <= N) __builtin_memcpy(p, &w, 16);
+    else {
+      const uint32_t d[4] = {w.x, w.y, w.z, w.w};
+      for (int j = 0; j < N - n0 - c; ++j) {
+        if (es == 4) ((uint32_t*)p)[j] = j == 0 ? d[0] : j == 1 ? d[1] : d[2];
+        else ((uint16_t*)p)[j] = (uint16_t)((j < 2 ? d[0] : j < 4 ? d[1] : j < 6 ? d[2] : d[3]) >> (16 * (j & 1)));
+      }
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+}
+
+struct Fp8NT {
+  const uint8_t* a; int64_t lda; const uint8_t* sa; int64_t ldsa;   // [M, K] rows of y
+  const uint8_t* b; int64_t ldb; const uint8_t* sb; int64_t ldsb;   // [N, K] columns of y
+  int64_t M; int N, nkb;                                            // nkb: blocks of 128 along K
+  int splits, per;                                                  // K in `splits` parts of `per` blocks; part s writes slab s of y (fp32, M x N each)
+  Fp8Out o;
+};
+
+// y = A B^T.  A tile of 128-byte rows lies in LDS with its 16-byte pieces turned by the row number (piece c of row r in slot c ^ (r & 7)), on
+// both sides of the direct global -> LDS copy: reads of 32 rows then meet every bank evenly.  Which bytes of a 128-block meet in which lane of
+// the matrix instruction is free (both operands use the same order and the block has one scale), so a lane takes pieces 4 h .. 4 h + 3.
+// WIDE: the fp32 results' form, 16-bit operands out of the same tiles.
+template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI>
+__global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
+  constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, ROWS = BM + BN;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];    // [2][ROWS][128]
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  const int wm = wave % WM, wn = wave / WM;
+  // blocks b and b + 8 run on the same XCD: the column tiles of a row tile go there back to back and find its rows in that L2
+  const int ntn = (p.N + BN - 1) / BN, xcd = blockIdx.x & 7, jj = blockIdx.x >> 3;
+  const int64_t m0 = ((int64_t)(jj / ntn) * 8 + xcd) * BM;
+  const int n0 = (jj % ntn) * BN;
+  if (m0 >= p.M) return;
+  const int kb0 = blockIdx.y * p.per, kb1 = min(p.nkb, kb0 + p.per);
+  f32x16 acc[NI][MI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  const int sub = lane >> 3, slot = lane & 7;
+  auto fetch = [&](int kb, int buf) {
+#pragma unroll
+    for (int i = 0; i < ROWS / 8 / NW; ++i) {
+      const int row = (wave + i * NW) * 8 + sub;       // row of the tile: A's first, then B's (a wave's eight rows are all of one kind)
+      const uint8_t* src = row < BM ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (int64_t)min(n0 + row - BM, p.N - 1) * p.ldb;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (int64_t)kb * 128 + ((slot ^ (row & 7)) * 16)),
+                                       (__attribute__((address_space(3))) void*)(smem8 + buf * ROWS * 128 + (wave + i * NW) * 1024), 16, 0, 0);
+    }
+  };
+  const uint8_t *pa[MI], *pb[NI];
+#pragma unroll
+  for (int j = 0; j < MI; ++j) pa[j] = p.sa + min(m0 + (wm * MI + j) * 32 + r, p.M - 1) * p.ldsa;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) pb[i] = p.sb + (int64_t)min(n0 + (wn * NI + i) * 32 + r, p.N - 1) * p.ldsb;
+  int sa[MI], sb[NI];
+  auto scales = [&](int kb) {
+#pragma unroll
+    for (int j = 0; j < MI; ++j) sa[j] = pa[j][kb];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sb[i] = pb[i][kb];
+  };
+  if (kb0 < kb1) {
+    fetch(kb0, 0);
+    __syncthreads();
+    for (int kb = kb0; kb < kb1; ++kb) {
+      const int buf = (kb - kb0) & 1;
+      scales(kb);
+      if (kb + 1 < kb1) fetch(kb + 1, buf ^ 1);
+      const uint8_t* t = smem8 + buf * ROWS * 128;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        i32x8 fa[MI], fb[NI];
+        const int c0 = 4 * h + 2 * ks;
+#pragma unroll
+        for (int j = 0; j < MI; ++j) {
+          const uint8_t* row = t + ((wm * MI + j) * 32 + r) * 128;
+          const i32x4 lo = *(const i32x4*)(row + ((c0 ^ (r & 7)) * 16)), hi = *(const i32x4*)(row + (((c0 + 1) ^ (r & 7)) * 16));
+          fa[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const uint8_t* row = t + (BM + (wn * NI + i) * 32 + r) * 128;
+          const i32x4 lo = *(const i32x4*)(row + ((c0 ^ (r & 7)) * 16)), hi = *(const i32x4*)(row + (((c0 + 1) ^ (r & 7)) * 16));
+          fb[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        }
+        if constexpr (WIDE) {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            b16x8 xa[MI];
+#pragma unroll
+            for (int j = 0; j < MI; ++j) xa[j] = widen8<FA>(fa[j][2 * q], fa[j][2 * q + 1], __uint_as_float((uint32_t)sa[j] << 23));
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+              const b16x8 xb = widen8<FB>(fb[i][2 * q], fb[i][2 * q + 1], __uint_as_float((uint32_t)sb[i] << 23));
+#pragma unroll
+              for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb, xa[j], acc[i][j], 0, 0, 0);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int j = 0; j < MI; ++j) acc[i][j] = mfma8<FB, FA>(fb[i], fa[j], acc[i][j], sb[i], sa[j]);
+        }
+      }
+      __syncthreads();          // the tile has been read, the next one has landed
+    }
+  }
+  Fp8Out o = p.o;
+  if (p.splits > 1) { o.y = (float*)o.y + (int64_t)blockIdx.y * p.M * p.N; o.ldy = p.N; o.type = FT_F32; o.relu = 0; }
+  uint8_t* buf = smem8 + wave * (32 * 272);
+#pragma unroll
+  for (int j = 0; j < MI; ++j)
+#pragma unroll
+    for (int i = 0; i < NI; i += 2) store_block(o, acc[i][j], acc[i + 1][j], buf, m0 + (wm * MI + j) * 32, p.M, n0 + (wn * NI + i) * 32, p.N, lane);
+}
+
+// the slabs of a split contraction, added in their order and rounded once
+__global__ __launch_bounds__(256) void k_fp8_join(const float* __restrict__ slabs, int splits, int64_t M, int N, Fp8Out o) {
+  const int64_t n = M * N;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
+    float s = 0.f;
+    for (int k = 0; k < splits; ++k) s += slabs[k * n + i];
+    if (o.relu) s = s < 0.f ? 0.f : s;
+    const int64_t at = i / N * o.ldy + i % N;
+    if (o.type == FT_F32) ((float*)o.y)[at] = s;
+    else if (o.type == FT_F16) ((h16*)o.y)[at] = (h16)s;
+    else ((__bf16*)o.y)[at] = (__bf16)s;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------------------ entry points
+static bool is_ft(int t) { return t >= FT_F16 && t <= FT_F32; }
+static bool is_f8(int f) { return f == F8_E4M3 || f == F8_E5M2; }
+static bool blocks_ok(const void* q, int64_t ldq, const void* s, int64_t lds, int64_t K) {
+  return q && s && ldq >= ceil128(K) && ldq % 16 == 0 && ((uintptr_t)q & 15) == 0 && lds >= ceil128(K) / 128 && lds % 4 == 0 && ((uintptr_t)s & 3) == 0;
+}
+#define FP8_BAD_BLOCKS "%s: 8-bit blocks need 16-byte aligned values with a pitch that is a multiple of 16 and holds whole blocks of 128, and 4-byte aligned scales with a pitch that is a multiple of 4"
+
+template <int T, int FMT>
+static int quant_launch(bool t, const void* x, int64_t ldx, int64_t M, int K, void* q, int64_t ldq, uint8_t* scale, int64_t lds, hipStream_t st) {
+  if (!t) {
+    const int nb = (int)(ceil128(K) / 128);
+    hipLaunchKernelGGL((k_fp8_quant<T, FMT>), dim3(aln_grid_for(M * nb, 16, 256 * 16)), dim3(256), 0, st, x, ldx, M, K, nb, (uint8_t*)q, ldq, scale, lds);
+  } else {
+    const int64_t nb = ceil128(M) / 128, g = nb * ((K + 63) / 64);
+    ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_quantize: %lld x %d values are too many for one launch", (long long)M, K);
+    hipLaunchKernelGGL((k_fp8_quant_t<T, FMT>), dim3((uint32_t)g), dim3(256), 0, st, x, ldx, M, K, (int)nb, (uint8_t*)q, ldq, scale, lds);
+  }
+  ALN_CHECK_LAUNCH("fp8_quantize");
+  return 0;
+}
+template <int T>
+static int quant_fmt(int fmt, bool t, const void* x, int64_t ldx, int64_t M, int K, void* q, int64_t ldq, uint8_t* scale, int64_t lds, hipStream_t st) {
+  return fmt == F8_E4M3 ? quant_launch<T, F8_E4M3>(t, x, ldx, M, K, q, ldq, scale, lds, st) : quant_launch<T, F8_E5M2>(t, x, ldx, M, K, q, ldq, scale, lds, st);
+}
+static int quantize(const char* name, bool t, const void* x, int x_type, int64_t ldx, int64_t M, int K, int fmt, void* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                    hipStream_t st) {
+  ALN_REQUIRE(is_ft(x_type) && is_f8(fmt), "%s: unknown type %d or format %d", name, x_type, fmt);
+  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && K >= 1 && ldx >= 0, "%s: %lld x %d values with pitch %lld", name, (long long)M, K, (long long)ldx);
+  if (M == 0) return 0;
+  ALN_REQUIRE(x, "%s: NULL pointer", name);
+  ALN_REQUIRE(((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0, "%s: x is not aligned to its type", name);
+  ALN_REQUIRE(blocks_ok(q, ldq, scale, lds, t ? M : K), FP8_BAD_BLOCKS, name);
+  return x_type == FT_F16 ? quant_fmt<FT_F16>(fmt, t, x, ldx, M, K, q, ldq, scale, lds, st) : x_type == FT_BF16 ? quant_fmt<FT_BF16>(fmt, t, x, ldx, M, K, q, ldq, scale, lds, st)
+                                                                                                : quant_fmt<FT_F32>(fmt, t, x, ldx, M, K, q, ldq, scale, lds, st);
+}
+extern "C" int aln_fp8_quantize(const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t K, int32_t fmt, void* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                                void* stream) {
+  return quantize("fp8_quantize", false, x, x_type, ldx, M, K, fmt, q, ldq, scale, lds, (hipStream_t)stream);
+}
+extern "C" int aln_fp8_quantize_t(const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t C, int32_t fmt, void* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                                  void* stream) {
+  return quantize("fp8_quantize_t", true, x, x_type, ldx, M, C, fmt, q, ldq, scale, lds, (hipStream_t)stream);
+}
+
+// How a product is cut: tiles of y, and parts of the contraction where the tiles alone leave most of the 256 CUs without work.
+struct NtPlan { int splits, per; };
+static NtPlan nt_plan(int64_t M, int N, int64_t K) {
+  const int64_t tiles = (M + 127) / 128 * ((N + 127) / 128), nkb = ceil128(K) / 128;
+  int64_t s = tiles >= 256 ? 1 : 512 / tiles;
+  if (s > nkb / 4) s = nkb / 4;
+  if (s < 1) s = 1;
+  const int64_t per = (nkb + s - 1) / s;
+  return {(int)((nkb + per - 1) / per), (int)per};
+}
+extern "C" int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  const NtPlan pl = nt_plan(M, N, K);
+  return pl.splits > 1 ? (int64_t)pl.splits * M * N * 4 : 0;
+}
+template <int FA, int FB, bool WIDE> static int nt_launch(Fp8NT& p, hipStream_t st) {
+  constexpr int WM = 2, WN = 2, MI = 2, NI = 2, BM = WM * MI * 32, BN = WN * NI * 32;
+  const int64_t g = ((p.M + BM - 1) / BM + 7) / 8 * 8 * ((p.N + BN - 1) / BN);
+  ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_nt: %lld x %d results are too many for one launch", (long long)p.M, p.N);
+  hipLaunchKernelGGL((k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>), dim3((uint32_t)g, p.splits), dim3(64 * WM * WN), 2 * (BM + BN) * 128, st, p);
+  ALN_CHECK_LAUNCH("fp8_nt");
+  return 0;
+}
+template <int FA, int FB> static int nt_type(Fp8NT& p, int y_type, hipStream_t st) {
+  return y_type == FT_F32 ? nt_launch<FA, FB, true>(p, st) : nt_launch<FA, FB, false>(p, st);
+}
+extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t ldsa, int32_t fmt_a, const void* b, int64_t ldb, const uint8_t* sb, int64_t ldsb,
+                          int32_t fmt_b, int64_t M, int32_t N, int64_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws, int64_t ws_bytes,
+                          void* stream) {
+  ALN_REQUIRE(is_f8(fmt_a) && is_f8(fmt_b) && is_ft(y_type), "fp8_nt: unknown format %d, %d or type %d", fmt_a, fmt_b, y_type);
+  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && K < (int64_t)1 << 31 && ldy >= N, "fp8_nt: sizes %lld x %d x %lld, pitch %lld", (long long)M, N, (long long)K,
+              (long long)ldy);
+  if (M == 0) return 0;
+  ALN_REQUIRE(blocks_ok(a, lda, sa, ldsa, K) && blocks_ok(b, ldb, sb, ldsb, K), FP8_BAD_BLOCKS, "fp8_nt");
+  ALN_REQUIRE(y && ((uintptr_t)y & (y_type == FT_F32 ? 3 : 1)) == 0, "fp8_nt: y is NULL or not aligned to its type");
+  const NtPlan pl = nt_plan(M, N, K);
+  ALN_REQUIRE(ws_bytes >= aln_fp8_nt_ws_bytes(M, N, K) && (pl.splits == 1 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_nt: the workspace needs %lld bytes, aligned to 16",
+              (long long)aln_fp8_nt_ws_bytes(M, N, K));
+  const Fp8Out o{y, ldy, y_type, relu};
+  Fp8NT p{(const uint8_t*)a, lda, sa, ldsa, (const uint8_t*)b, ldb, sb, ldsb, M, N, (int)(ceil128(K) / 128), pl.splits, pl.per, o};
+  if (pl.splits > 1) p.o.y = ws;
+  hipStream_t st = (hipStream_t)stream;
+  const int rc = fmt_a == F8_E4M3 ? (fmt_b == F8_E4M3 ? nt_type<F8_E4M3, F8_E4M3>(p, y_type, st) : nt_type<F8_E4M3, F8_E5M2>(p, y_type, st))
+                                  : (fmt_b == F8_E4M3 ? nt_type<F8_E5M2, F8_E4M3>(p, y_type, st) : nt_type<F8_E5M2, F8_E5M2>(p, y_type, st));
+  if (rc || pl.splits == 1) return rc;
+  hipLaunchKernelGGL(k_fp8_join, dim3(aln_grid_for(M * N, 256, 2048)), dim3(256), 0, st, (const float*)ws, pl.splits, M, N, o);
+  ALN_CHECK_LAUNCH("fp8_nt");
+  return 0;
+}

@@ -1,0 +1,198 @@
+"""Linear layers in 8-bit floating point with one power-of-two scale per block of 128 (csrc/fp8.hip), and their gradients.
+
+The wide feature heads (autolabel/models.py:117-136 at LSeg width) and the compression autoencoder (autolabel/models.py:268-294) are matrix
+products over up to a million rows; the reference runs them in fp16.  Here an operand is cut into blocks of 128 along the contracted axis and
+each block is held as 8-bit values (``'e4m3'``, or ``'e5m2'`` with more range and a bit less precision) times one power of two, chosen so that
+nothing is clipped; the products run on the block-scaled matrix instructions and accumulate in fp32.
+
+    w = fp8.quantize(weight)                 # [out, in], once
+    y = fp8.linear(x, w, relu=True)          # x [..., in] fp16 / bf16 / fp32 -> [..., out]
+    dx, dw = fp8.linear_backward(g, x, fp8.quantize(weight.t()))
+
+``Linear`` wraps the three for autograd.  Every call allocates its results and its scratch from torch's allocator and enqueues on the current
+stream of the tensors' device; nothing is kept between calls and nothing synchronises, so the calls can be captured into a graph.
+"""
+import contextlib
+from dataclasses import dataclass
+
+import torch
+
+from . import hip as H
+
+BLOCK = 128
+FORMATS = {'e4m3': (0, torch.float8_e4m3fn), 'e5m2': (1, torch.float8_e5m2)}
+TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+
+
+def _blocks(n):
+    return (n + BLOCK - 1) // BLOCK
+
+
+@dataclass
+class Fp8Blocks:
+    """A matrix [rows, cols] in 8-bit blocks: ``q`` [rows, >= 128 ceil(cols / 128)] of the 8-bit type (zeros behind column ``cols``) and
+    ``scale`` [rows, a multiple of 4 >= ceil(cols / 128)] uint8, exponent + 127 of each block's power of two."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    cols: int
+    fmt: str = 'e4m3'
+
+    @property
+    def rows(self):
+        return self.q.shape[0]
+
+    def dequantize(self):
+        """The values the blocks stand for, [rows, cols] fp32 (torch operations: for inspection)."""
+        s = ((self.scale.int()) << 23).view(torch.float32)[:, :_blocks(self.cols)]
+        return (self.q.float()[:, :_blocks(self.cols) * BLOCK].reshape(self.rows, -1, BLOCK) * s[..., None]).reshape(self.rows, -1)[:, :self.cols]
+
+    def _check(self, name):
+        if self.fmt not in FORMATS:
+            raise ValueError(f'{name}: unknown 8-bit format {self.fmt!r} (one of {", ".join(FORMATS)})')
+        nb = _blocks(self.cols)
+        q, s = self.q, self.scale
+        if self.cols < 1 or q.dim() != 2 or q.dtype != FORMATS[self.fmt][1] or not q.is_contiguous() or q.shape[1] < nb * BLOCK or q.shape[1] % 16:
+            raise ValueError(f'{name}: q must be contiguous {FORMATS[self.fmt][1]} [rows, whole blocks of 128 for {self.cols} columns], got {q.dtype} {tuple(q.shape)}')
+        if s.dim() != 2 or s.dtype != torch.uint8 or not s.is_contiguous() or s.shape[0] != q.shape[0] or s.shape[1] < nb or s.shape[1] % 4 or s.device != q.device:
+            raise ValueError(f'{name}: scale must be contiguous uint8 [rows, a multiple of 4 >= {nb}] beside q, got {s.dtype} {tuple(s.shape)}')
+
+
+def _need(ok, message):
+    if not ok:
+        raise ValueError(message)
+
+
+def _rows(name, x):
+    """x as [rows, columns] with unit column stride (a view where its strides allow one, else a copy)."""
+    _need(torch.is_tensor(x) and x.dtype in TYPES, f'{name}: needs an fp16, bf16 or fp32 tensor')
+    _need(x.dim() >= 1 and x.shape[-1] >= 1, f'{name}: needs at least one column, got shape {tuple(x.shape)}')
+    x = x.detach()
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    if x.shape[1] > 1 and x.stride(1) != 1:
+        x = x.contiguous()
+    return x
+
+
+def _pitch(x):
+    return x.stride(0) if x.shape[0] > 1 else x.shape[1]
+
+
+def _on(*tensors):
+    """The tensors' common device made current (a no-op where it is)."""
+    dev = tensors[0].device
+    for t in tensors:
+        _need(t.is_cuda, 'autolabel_amd.fp8 has no CPU path: needs device tensors')
+        _need(t.device == dev, f'tensors on different devices: {dev} and {t.device}')
+    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _p(t):
+    return t.data_ptr()
+
+
+def _empty_blocks(rows, cols, fmt, device):
+    nb = _blocks(cols)
+    return Fp8Blocks(torch.empty(rows, nb * BLOCK, dtype=FORMATS[fmt][1], device=device),
+                     torch.empty(rows, (nb + 3) // 4 * 4, dtype=torch.uint8, device=device), cols, fmt)
+
+
+def quantize(x, fmt='e4m3', transpose=False):
+    """Blocks of ``x`` [..., K] along its last axis -> Fp8Blocks of [rows, K]; ``transpose=True``: blocks of x^T along the rows of x ->
+    Fp8Blocks of [K, rows] (what a product over the rows needs)."""
+    _need(fmt in FORMATS, f'quantize: unknown 8-bit format {fmt!r} (one of {", ".join(FORMATS)})')
+    x = _rows('quantize', x)
+    m, k = x.shape
+    _need(m >= 1 or not transpose, 'quantize: x^T of an empty x has no columns')
+    with _on(x):
+        out = _empty_blocks(k, m, fmt, x.device) if transpose else _empty_blocks(m, k, fmt, x.device)
+        H.call('aln_fp8_quantize_t' if transpose else 'aln_fp8_quantize', _p(x), TYPES[x.dtype], _pitch(x), m, k, FORMATS[fmt][0], _p(out.q),
+               out.q.shape[1], _p(out.scale), out.scale.shape[1], H.stream())
+    return out
+
+
+def _out_type(name, dtype):
+    _need(dtype in TYPES, f'{name}: results are fp16, bf16 or fp32, not {dtype}')
+    return dtype
+
+
+def matmul(a, b, out_dtype=torch.float16, relu=False):
+    """a [M, K] b [N, K]^T of two Fp8Blocks -> [M, N], accumulated in fp32 and rounded once."""
+    a._check('matmul: a'); b._check('matmul: b')
+    _need(a.cols == b.cols, f'matmul: the operands contract over {a.cols} and {b.cols} columns')
+    _need(b.rows >= 1, 'matmul: b has no rows')
+    _out_type('matmul', out_dtype)
+    m, n, k = a.rows, b.rows, a.cols
+    with _on(a.q, b.q):
+        y = torch.empty(m, n, dtype=out_dtype, device=a.q.device)
+        nbytes = int(H.lib().aln_fp8_nt_ws_bytes(m, n, k))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=a.q.device) if nbytes else None
+        H.call('aln_fp8_nt', _p(a.q), a.q.shape[1], _p(a.scale), a.scale.shape[1], FORMATS[a.fmt][0], _p(b.q), b.q.shape[1], _p(b.scale),
+               b.scale.shape[1], FORMATS[b.fmt][0], m, n, k, _p(y), n, TYPES[out_dtype], int(bool(relu)), _p(ws) if nbytes else None, nbytes, H.stream())
+    return y
+
+
+def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
+    """x [..., K] W^T for ``weight`` = Fp8Blocks of W [N, K] -> [..., N] of x's type (or ``out_dtype``); the rows of x are cut into blocks of
+    ``fmt`` on the way.  ``relu``: negative results become 0."""
+    _need(isinstance(weight, Fp8Blocks), 'linear: weight must be Fp8Blocks (fp8.quantize)')
+    weight._check('linear: weight')
+    _need(fmt in FORMATS, f'linear: unknown 8-bit format {fmt!r} (one of {", ".join(FORMATS)})')
+    rows = _rows('linear', x)
+    _need(rows.shape[1] == weight.cols, f'linear: x has {rows.shape[1]} columns, the weight {weight.cols}')
+    out_dtype = _out_type('linear', out_dtype or x.dtype)
+    return matmul(quantize(rows, fmt), weight, out_dtype, relu).reshape(*x.shape[:-1], weight.rows)
+
+
+def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True):
+    """Gradients of y = x W^T (no activation) from ``g`` = dL/dy [..., N] and ``x`` [..., K]: (dL/dx of x's type, dL/dW [N, K] fp32), either
+    one None where not needed.  ``weight_t`` = Fp8Blocks of W^T [K, N] (not read for dL/dW alone: may be None then).  g is cut into blocks of
+    ``grad_fmt`` along N for dL/dx, g and x along their rows for dL/dW; the sums over the rows are taken in a fixed order."""
+    _need(grad_fmt in FORMATS, f'linear_backward: unknown 8-bit format {grad_fmt!r} (one of {", ".join(FORMATS)})')
+    gr, xr = _rows('linear_backward: g', g), _rows('linear_backward: x', x)
+    _need(g.shape[:-1] == x.shape[:-1], f'linear_backward: g has the rows {tuple(g.shape[:-1])}, x {tuple(x.shape[:-1])}')
+    if need_dx:
+        _need(isinstance(weight_t, Fp8Blocks), 'linear_backward: weight_t must be Fp8Blocks (fp8.quantize of the transposed weight)')
+        weight_t._check('linear_backward: weight_t')
+        _need(weight_t.rows == xr.shape[1] and weight_t.cols == gr.shape[1],
+              f'linear_backward: weight_t is {weight_t.rows} x {weight_t.cols}, x has {xr.shape[1]} columns and g {gr.shape[1]}')
+    dx = dw = None
+    if need_dx:
+        dx = linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt).reshape(x.shape)
+    if need_dw:
+        with _on(gr, xr):
+            if gr.shape[0] == 0:
+                dw = torch.zeros(gr.shape[1], xr.shape[1], device=x.device)
+            else:
+                dw = matmul(quantize(gr, grad_fmt, transpose=True), quantize(xr, transpose=True), torch.float32)
+    return dx, dw
+
+
+class _LinearFunction(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, x, weight, grad_fmt):
+        ctx.save_for_backward(x, weight)
+        ctx.grad_fmt = grad_fmt
+        return linear(x, quantize(weight))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        x, weight = ctx.saved_tensors
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        dx, dw = linear_backward(g, x, quantize(weight.detach().t()) if need_dx else None, ctx.grad_fmt, need_dx, need_dw)
+        return dx, None if dw is None else dw.to(weight.dtype), None
+
+
+class Linear(torch.nn.Linear):
+    """``torch.nn.Linear`` without a bias whose three products run in 8-bit blocks: the same parameter, initialisation and state_dict, the
+    weight kept in its own type and cut into blocks at every call (it changes with every optimizer step)."""
+
+    def __init__(self, in_features, out_features, grad_fmt='e4m3', device=None, dtype=None):
+        _need(grad_fmt in FORMATS, f'Linear: unknown 8-bit format {grad_fmt!r} (one of {", ".join(FORMATS)})')
+        super().__init__(in_features, out_features, bias=False, device=device, dtype=dtype)
+        self.grad_fmt = grad_fmt
+
+    def forward(self, x):
+        return _LinearFunction.apply(x, self.weight, self.grad_fmt)

@@ -446,6 +446,38 @@ int aln_grad_unpack_f16(const void* in_f16, int64_t n, float* grad, int32_t* fou
 /* staging for a reduce-scatter: as aln_grad_pack_f16, plus out[n, n_pad) = 0 and grad[0, n) cleared behind the read */
 int aln_grad_pack_f16_clear(float* grad, int64_t n, int64_t n_pad, float mul, void* out_f16, void* stream);
 
+/* ---- products in 8-bit floating point, one power-of-two scale per block of 128 along the contracted axis (fp8.hip; no counterpart in
+ * the reference, whose heads run in fp16).  Beside aln_wide_nt / aln_wide_tn for layers whose operands may be 8 bits wide.
+ * Types (x_type, y_type): 0 fp16, 1 bf16, 2 fp32.  Formats (fmt): 0 e4m3 (largest 448), 1 e5m2 (largest 57344).
+ * A matrix [R, K] in blocks: q [R, ldq] bytes, ldq a multiple of 16 and >= 128 ceil(K / 128), zero behind column K; scale [R, lds] bytes
+ * holding exponent + 127, lds a multiple of 4: x[r][k] ~ q[r][k] * 2^(scale[r][k / 128] - 127).  q 16-byte, scale 4-byte aligned.
+ * aln_fp8_quantize: blocks of x [M, K], row pitch ldx elements (x aligned to its type only).  The scale is the smallest power of two
+ * >= 2^-126 that brings the block's largest magnitude into the format's range (1 for zeros), the values are rounded to nearest even: nothing
+ * is clipped.  A block holding an infinity or a NaN becomes NaN throughout.
+ * aln_fp8_quantize_t: blocks of x^T, x [M, C]: q [C, ldq], blocks of 128 along M -- the operands of a product over the rows of x. */
+int aln_fp8_quantize(const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t K, int32_t fmt, void* q, int64_t ldq, uint8_t* scale,
+                     int64_t lds, void* stream);
+int aln_fp8_quantize_t(const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t C, int32_t fmt, void* q, int64_t ldq, uint8_t* scale,
+                       int64_t lds, void* stream);
+/* y [M, N] = A [M, K] B [N, K]^T, both in blocks, accumulated in fp32 and rounded once to y_type; relu: negative results become 0 (NaN
+ * stays).  ws: aln_fp8_nt_ws_bytes(M, N, K) bytes, 16-byte aligned (0: may be NULL): a long contraction with few results is split, the parts
+ * are added in a fixed order. */
+int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K);
+int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t ldsa, int32_t fmt_a, const void* b, int64_t ldb, const uint8_t* sb,
+               int64_t ldsb, int32_t fmt_b, int64_t M, int32_t N, int64_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws,
+               int64_t ws_bytes, void* stream);
+
+/* ---- global gradient norm and clipping (clip.hip; no counterpart in the reference, whose optimizer step is autolabel/trainer.py:45-48
+ * without one).  n tensors of numel[k] elements (host arrays; types[k]: 0 fp16, 1 bf16, 2 fp32; device pointers aligned to their type):
+ *   norm = sqrt(sum of all squares, in fp64) / loss_scale;  out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)), rounded to the tensor's type
+ * out NULL or out[k] == grads[k]: in place (nothing is written when the factor is 1).  No two tensors may share memory otherwise.
+ * apply = 0: the norm only.  loss_scale (device float), norm (device float), found_inf (device word) may be NULL.  A norm that is not finite
+ * in fp32 scales nothing and raises *found_inf.  Bit-reproducible.  ws: aln_grad_clip_ws_bytes(n) bytes, 8-byte aligned. */
+int64_t aln_grad_clip_ws_bytes(int32_t n);
+int aln_grad_clip(int32_t n, const void* const* grads /*host*/, void* const* out /*host*/, const int64_t* numel /*host*/,
+                  const int32_t* types /*host*/, float max_norm, int32_t apply, const float* loss_scale, float* norm, int32_t* found_inf, void* ws,
+                  int64_t ws_bytes, void* stream);
+
 /* ---- feature-map file: autolabel/dataset.py:438-441 reads features.hdf through h5py, whose LZF filter (id 32000,
  * scripts/compute_feature_maps.py:85) wraps liblzf.  HOST pointers; returns the number of bytes produced or -1. */
 int64_t aln_lzf_decompress(const void* src /*host*/, size_t n_in, void* dst /*host*/, size_t n_out);
