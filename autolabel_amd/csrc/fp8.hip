@@ -201,6 +201,7 @@ template <int FA, int FB> __device__ inline f32x16 mfma8(i32x8 a, i32x8 b, f32x1
 
 // two 8-bit values (the upper two of the word with HI) times a power of two, exact in bf16
 typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 template <int FMT, bool HI> __device__ inline b16x2 widen2(uint32_t w, float s) {
   if constexpr (FMT == F8_E4M3) return __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, s, HI);
@@ -215,39 +216,45 @@ struct Fp8Out { void* y; int64_t ldy; int type, relu; };   // type: FT_*
 
 // One wave's 32 x 64 block of the result.  The accumulators hold D[n][m]: lane = row m of y (lane % 32), register r = column
 // 8 (r / 4) + 4 (lane / 32) + r % 4 -- stores from there would touch 32 rows per instruction with 8 bytes each, so the block, already rounded
-// to its type, goes round through LDS (`buf`, the wave's own 32 x 272 bytes) and leaves row by row, 16 bytes a lane.
+// to its type, goes round through LDS (`buf`, the wave's own 4 KB, fp32 8 KB; 16-byte pieces turned by the row against bank conflicts) and
+// leaves row by row, 16 bytes a lane.
+template <bool F32>
 __device__ inline void store_block(const Fp8Out& o, const f32x16& c0, const f32x16& c1, uint8_t* buf, int64_t m0, int64_t M, int n0, int N, int lane) {
-  const int r = lane & 31, h = lane >> 5, es = o.type == FT_F32 ? 4 : 2, pitch = 64 * es + 16;
+  constexpr int ES = F32 ? 4 : 2, PIECES = 4 * ES, PER = 16 / ES;      // pieces of 16 bytes per row of 64, values per piece
+  const int r = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int s = 0; s < 2; ++s)
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-      float v[4];
+      f32x4 v = s ? (f32x4){c1[4 * g], c1[4 * g + 1], c1[4 * g + 2], c1[4 * g + 3]} : (f32x4){c0[4 * g], c0[4 * g + 1], c0[4 * g + 2], c0[4 * g + 3]};
+      if (o.relu) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) { v[j] = s ? c1[4 * g + j] : c0[4 * g + j]; if (o.relu) v[j] = v[j] < 0.f ? 0.f : v[j]; }   // (a NaN stays)
-      const int col = 32 * s + 8 * g + 4 * h;
-      if (o.type == FT_F32) *(f32x4*)(buf + r * pitch + 4 * col) = (f32x4){v[0], v[1], v[2], v[3]};
-      else if (o.type == FT_F16) *(h16x4*)(buf + r * pitch + 2 * col) = (h16x4){(h16)v[0], (h16)v[1], (h16)v[2], (h16)v[3]};
+        for (int j = 0; j < 4; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];       // (a NaN stays)
+      }
+      if constexpr (F32) *(f32x4*)(buf + r * 256 + (((8 * s + 2 * g + h) ^ (r & 15)) * 16)) = v;
       else {
-        typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
-        *(b16x4*)(buf + r * pitch + 2 * col) = (b16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        uint8_t* q = buf + r * 128 + (((4 * s + g) ^ (r & 7)) * 16) + 8 * h;
+        if (o.type == FT_F16) *(h16x4*)q = (h16x4){(h16)v[0], (h16)v[1], (h16)v[2], (h16)v[3]};
+        else *(b16x4*)q = (b16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
       }
     }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
   __builtin_amdgcn_wave_barrier();
-  const int lpr = 4 * es, per = 16 / es;            // lanes per row of 64 values, values per lane
-  for (int i = lane; i < 32 * lpr; i += 64) {
-    const int row = i / lpr, c = (i % lpr) * per;
+#pragma unroll
+  for (int it = 0; it < PIECES / 2; ++it) {
+    const int row = it * (64 / PIECES) + lane / PIECES, piece = lane % PIECES, c = piece * PER;
     const int64_t m = m0 + row;
+    const uint4 w = *(const uint4*)(buf + row * 16 * PIECES + ((piece ^ (row & (F32 ? 15 : 7))) * 16));
     if (m >= M || n0 + c >= N) continue;
-    const uint4 w = *(const uint4*)(buf + row * pitch + c * es);
-    uint8_t* p = (uint8_t*)o.y + (m * o.ldy + n0 + c) * es;
-    if (n0 + c + per <= N) __builtin_memcpy(p, &w, 16);
+    uint8_t* p = (uint8_t*)o.y + (m * o.ldy + n0 + c) * ES;
+    if (n0 + c + PER <= N) __builtin_memcpy(p, &w, 16);
     else {
       const uint32_t d[4] = {w.x, w.y, w.z, w.w};
-      for (int j = 0; j < N - n0 - c; ++j) {
-        if (es == 4) ((uint32_t*)p)[j] = j == 0 ? d[0] : j == 1 ? d[1] : d[2];
-        else ((uint16_t*)p)[j] = (uint16_t)((j < 2 ? d[0] : j < 4 ? d[1] : j < 6 ? d[2] : d[3]) >> (16 * (j & 1)));
+#pragma unroll
+      for (int j = 0; j < PER - 1; ++j) {
+        if (n0 + c + j >= N) continue;
+        if constexpr (F32) ((uint32_t*)p)[j] = d[j];
+        else ((uint16_t*)p)[j] = (uint16_t)(d[j / 2] >> (16 * (j & 1)));
       }
     }
   }
@@ -356,11 +363,107 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
   }
   Fp8Out o = p.o;
   if (p.splits > 1) { o.y = (float*)o.y + (int64_t)blockIdx.y * p.M * p.N; o.ldy = p.N; o.type = FT_F32; o.relu = 0; }
-  uint8_t* buf = smem8 + wave * (32 * 272);
+  uint8_t* buf = smem8 + wave * 8192;
 #pragma unroll
   for (int j = 0; j < MI; ++j)
 #pragma unroll
-    for (int i = 0; i < NI; i += 2) store_block(o, acc[i][j], acc[i + 1][j], buf, m0 + (wm * MI + j) * 32, p.M, n0 + (wn * NI + i) * 32, p.N, lane);
+    for (int i = 0; i < NI; i += 2) {
+      if (o.type == FT_F32) store_block<true>(o, acc[i][j], acc[i + 1][j], buf, m0 + (wm * MI + j) * 32, p.M, n0 + (wn * NI + i) * 32, p.N, lane);
+      else store_block<false>(o, acc[i][j], acc[i + 1][j], buf, m0 + (wm * MI + j) * 32, p.M, n0 + (wn * NI + i) * 32, p.N, lane);
+    }
+}
+
+// y = x W^T with the rows of x cut into blocks on the way: 64 rows of x, all of their (up to 1024) columns, become 8-bit values in LDS once,
+// then the weights stream past them from L2 in tiles of 128 rows x 128 columns -- the values of x never exist in 8 bits in memory.
+struct Fp8Linear {
+  const void* x; int64_t ldx;
+  const uint8_t* w; int64_t ldw; const uint8_t* sw; int64_t ldsw;
+  int64_t M; int N, K, nkb;
+  int parts, per;                 // the columns of y in `parts` parts of `per` tiles of 128
+  Fp8Out o;
+};
+#define LIN_BM 64
+#define LIN_NKB 8
+static inline int lin_lds(int nkb) { return LIN_BM * nkb * 128 + 2 * 128 * 128 + LIN_BM * LIN_NKB; }
+
+template <int T, int FX, int FW>
+__global__ __launch_bounds__(256) void k_fp8_linear(Fp8Linear p) {
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];
+  uint8_t* xs = smem8;                                    // [64][nkb][128], pieces of 16 bytes turned by the row within each block
+  uint8_t* ws = xs + LIN_BM * p.nkb * 128;                // [2][128][128]
+  uint8_t* se = ws + 2 * 128 * 128;                       // [64][8] exponents + 127
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  const int wm = wave & 1, wn = wave >> 1;
+  // blocks b and b + 8 run on the same XCD: the parts of a row tile go there and share its rows in that L2
+  const int xcd = blockIdx.x & 7, jj = blockIdx.x >> 3;
+  const int64_t m0 = ((int64_t)(jj / p.parts) * 8 + xcd) * LIN_BM;
+  if (m0 >= p.M) return;
+  const int t0 = (jj % p.parts) * p.per, t1 = min((p.N + 127) / 128, t0 + p.per);
+  const int steps = (t1 - t0) * p.nkb;
+  const int sub = lane >> 3, slot = lane & 7;
+  auto fetch = [&](int step) {
+    const int t = t0 + step / p.nkb, kb = step % p.nkb;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = (wave * 4 + i) * 8 + sub;
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p.w + (int64_t)min(t * 128 + row, p.N - 1) * p.ldw + kb * 128 + ((slot ^ (row & 7)) * 16)),
+                                       (__attribute__((address_space(3))) void*)(ws + (step & 1) * 16384 + (wave * 4 + i) * 1024), 16, 0, 0);
+    }
+  };
+  if (steps > 0) fetch(0);
+  {
+    const int g = tid >> 4, s16 = tid & 15;               // 16 lanes a block of 128, 16 rows at a time
+    for (int b = 0; b < p.nkb; ++b) {
+      Eight<T> v[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { const int k = b * 128 + s16 * 8; v[i].load(p.x, min(m0 + 16 * i + g, p.M - 1) * p.ldx + k, p.K - k); }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = 16 * i + g;
+        float f;
+        const int e = block_exp<FX>(umax16(v[i].amax()), f);
+        *(uint2*)(xs + (row * p.nkb + b) * 128 + (((s16 >> 1) ^ (row & 7)) * 16) + (s16 & 1) * 8) = quant8<T, FX>(v[i], f);
+        if (s16 == 0) se[row * LIN_NKB + b] = (uint8_t)(e + 127);
+      }
+    }
+  }
+  __syncthreads();
+  f32x16 acc[2];
+  const int xrow = wm * 32 + r;
+  for (int step = 0; step < steps; ++step) {
+    const int t = t0 + step / p.nkb, kb = step % p.nkb;
+    if (step + 1 < steps) fetch(step + 1);
+    if (kb == 0) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
+    }
+    int sb[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sb[i] = p.sw[(int64_t)min(t * 128 + wn * 64 + i * 32 + r, p.N - 1) * p.ldsw + kb];
+    const int sa = se[xrow * LIN_NKB + kb];
+    const uint8_t* xr = xs + (xrow * p.nkb + kb) * 128;
+    const uint8_t* wt = ws + (step & 1) * 16384;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      const int c0 = 4 * h + 2 * ks, o0 = (c0 ^ (r & 7)) * 16, o1 = ((c0 + 1) ^ (r & 7)) * 16;
+      const i32x8 fx = __builtin_shufflevector(*(const i32x4*)(xr + o0), *(const i32x4*)(xr + o1), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint8_t* wr = wt + (wn * 64 + i * 32 + r) * 128;
+        const i32x8 fw = __builtin_shufflevector(*(const i32x4*)(wr + o0), *(const i32x4*)(wr + o1), 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[i] = mfma8<FW, FX>(fw, fx, acc[i], sb[i], sa);
+      }
+    }
+    __syncthreads();            // the tile has been read, the next one has landed
+    if (kb == p.nkb - 1) {
+      // the next tile has landed in the other half: this one's is free for the result
+      uint8_t* buf = ws + (step & 1) * 16384 + wave * 4096;
+      store_block<false>(p.o, acc[0], acc[1], buf, m0 + wm * 32, p.M, t * 128 + wn * 64, p.N, lane);
+      __syncthreads();
+    }
+  }
 }
 
 // the slabs of a split contraction, added in their order and rounded once
@@ -470,4 +573,53 @@ extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t
   hipLaunchKernelGGL(k_fp8_join, dim3(aln_grid_for(M * N, 256, 2048)), dim3(256), 0, st, (const float*)ws, pl.splits, M, N, o);
   ALN_CHECK_LAUNCH("fp8_nt");
   return 0;
+}
+
+// ---- x W^T for x as it is.  Up to 1024 columns and 16-bit results: the one-launch kernel; otherwise blocks of x in the workspace, then the product.
+static bool lin_fused(int64_t K, int y_type) { return ceil128(K) / 128 <= LIN_NKB && y_type != FT_F32; }
+static inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
+extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t y_type) {
+  if (M <= 0 || N <= 0 || K <= 0 || lin_fused(K, y_type)) return 0;
+  const int64_t nb = ceil128(K) / 128;
+  return M * nb * 128 + up16(M * ((nb + 3) / 4 * 4)) + aln_fp8_nt_ws_bytes(M, N, K);
+}
+template <int T, int FX, int FW> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
+  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_linear<T, FX, FW>, hipFuncAttributeMaxDynamicSharedMemorySize, lin_lds(LIN_NKB));
+  ALN_REQUIRE(big == hipSuccess, "fp8_linear: %s", hipGetErrorString(big));
+  const int64_t g = ((p.M + LIN_BM - 1) / LIN_BM + 7) / 8 * 8 * p.parts;
+  ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_linear: %lld x %d results are too many for one launch", (long long)p.M, p.N);
+  hipLaunchKernelGGL((k_fp8_linear<T, FX, FW>), dim3((uint32_t)g), dim3(256), lin_lds(p.nkb), st, p);
+  ALN_CHECK_LAUNCH("fp8_linear");
+  return 0;
+}
+template <int T> static int lin_fmt(int fx, int fw, const Fp8Linear& p, hipStream_t st) {
+  return fx == F8_E4M3 ? (fw == F8_E4M3 ? lin_launch<T, F8_E4M3, F8_E4M3>(p, st) : lin_launch<T, F8_E4M3, F8_E5M2>(p, st))
+                       : (fw == F8_E4M3 ? lin_launch<T, F8_E5M2, F8_E4M3>(p, st) : lin_launch<T, F8_E5M2, F8_E5M2>(p, st));
+}
+extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, const void* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, int32_t fmt_w,
+                              int64_t M, int32_t N, int32_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws, int64_t ws_bytes, void* stream) {
+  ALN_REQUIRE(is_ft(x_type) && is_ft(y_type) && is_f8(fmt_x) && is_f8(fmt_w), "fp8_linear: unknown type %d, %d or format %d, %d", x_type, y_type, fmt_x, fmt_w);
+  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldx >= 0 && ldy >= N, "fp8_linear: sizes %lld x %d x %d, pitches %lld, %lld", (long long)M, N, K,
+              (long long)ldx, (long long)ldy);
+  if (M == 0) return 0;
+  ALN_REQUIRE(blocks_ok(w, ldw, sw, ldsw, K), FP8_BAD_BLOCKS, "fp8_linear");
+  ALN_REQUIRE(x && ((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0 && y && ((uintptr_t)y & (y_type == FT_F32 ? 3 : 1)) == 0, "fp8_linear: x or y is NULL or not aligned to its type");
+  const int64_t need = aln_fp8_linear_ws_bytes(M, N, K, y_type);
+  ALN_REQUIRE(ws_bytes >= need && (need == 0 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_linear: the workspace needs %lld bytes, aligned to 16", (long long)need);
+  const int nkb = (int)(ceil128(K) / 128);
+  if (!lin_fused(K, y_type)) {
+    uint8_t* q = (uint8_t*)ws, *sc = q + M * nkb * 128, *rest = sc + up16(M * ((nkb + 3) / 4 * 4));
+    const int rc = aln_fp8_quantize(x, x_type, ldx, M, K, fmt_x, q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, stream);
+    if (rc) return rc;
+    return aln_fp8_nt(q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, fmt_x, w, ldw, sw, ldsw, fmt_w, M, N, K, y, ldy, y_type, relu, rest, ws_bytes - (rest - q), stream);
+  }
+  // parts: the columns of y are cut only while the row tiles leave CUs without work (a part cuts the tile's rows into blocks again)
+  const int64_t mt = (M + LIN_BM - 1) / LIN_BM;
+  const int nt = (N + 127) / 128;
+  int parts = (int)(mt >= 512 ? 1 : 512 / mt);
+  if (parts > nt) parts = nt;
+  const int per = (nt + parts - 1) / parts;
+  const Fp8Linear p{x, ldx, (const uint8_t*)w, ldw, sw, ldsw, M, N, K, nkb, (nt + per - 1) / per, per, Fp8Out{y, ldy, y_type, relu}};
+  hipStream_t st = (hipStream_t)stream;
+  return x_type == FT_F16 ? lin_fmt<FT_F16>(fmt_x, fmt_w, p, st) : x_type == FT_BF16 ? lin_fmt<FT_BF16>(fmt_x, fmt_w, p, st) : lin_fmt<FT_F32>(fmt_x, fmt_w, p, st);
 }

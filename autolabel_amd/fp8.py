@@ -141,7 +141,16 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
     rows = _rows('linear', x)
     _need(rows.shape[1] == weight.cols, f'linear: x has {rows.shape[1]} columns, the weight {weight.cols}')
     out_dtype = _out_type('linear', out_dtype or x.dtype)
-    return matmul(quantize(rows, fmt), weight, out_dtype, relu).reshape(*x.shape[:-1], weight.rows)
+    (m, k), n = rows.shape, weight.rows
+    _need(n >= 1, 'linear: the weight has no rows')
+    with _on(rows, weight.q):
+        y = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
+        nbytes = H.lib().aln_fp8_linear_ws_bytes(m, n, k, TYPES[out_dtype])
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+        H.call('aln_fp8_linear', _p(rows), TYPES[x.dtype], _pitch(rows), FORMATS[fmt][0], _p(weight.q), weight.q.shape[1], _p(weight.scale),
+               weight.scale.shape[1], FORMATS[weight.fmt][0], m, n, k, _p(y), n, TYPES[out_dtype], int(bool(relu)), _p(ws) if nbytes else None, nbytes,
+               H.stream())
+    return y
 
 
 def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True):

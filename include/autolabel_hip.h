@@ -467,6 +467,14 @@ int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t ldsa, int3
                int64_t ldsb, int32_t fmt_b, int64_t M, int32_t N, int64_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws,
                int64_t ws_bytes, void* stream);
 
+/* y [M, N] = x W^T for x [M, K] as it is (row pitch ldx): its rows are cut into blocks of fmt_x on the way -- the same result as
+ * aln_fp8_quantize + aln_fp8_nt up to the order of the fp32 additions.  ws: aln_fp8_linear_ws_bytes(M, N, K, y_type) bytes, 16-byte aligned
+ * (0: may be NULL). */
+int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t y_type);
+int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, const void* w, int64_t ldw, const uint8_t* sw, int64_t ldsw,
+                   int32_t fmt_w, int64_t M, int32_t N, int32_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws,
+                   int64_t ws_bytes, void* stream);
+
 /* ---- global gradient norm and clipping (clip.hip; no counterpart in the reference, whose optimizer step is autolabel/trainer.py:45-48
  * without one).  n tensors of numel[k] elements (host arrays; types[k]: 0 fp16, 1 bf16, 2 fp32; device pointers aligned to their type):
  *   norm = sqrt(sum of all squares, in fp64) / loss_scale;  out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)), rounded to the tensor's type
