@@ -39,14 +39,16 @@ __device__ inline uint32_t umax16(uint32_t v) {
   return dpp_umax<0x140>(v);  // row_mirror
 }
 
-// e of a block from the bits of max |x| as fp32 (NaN and infinity compare above every finite value), and the factor 2^-e (NaN for such a block)
-template <int FMT> __device__ inline int block_exp(uint32_t amax_bits, float& factor) {
+// A block's power of two 2^e from the bits of max |x| as fp32 (NaN and infinity compare above every finite value)
+struct BlockScale { uint8_t byte; bool finite; float scale, factor; };    // e + 127; 2^e; 2^-e, or NaN for a block that is not finite
+template <int FMT> __device__ inline BlockScale block_scale(uint32_t amax_bits) {
   constexpr int EMAX = FMT == F8_E4M3 ? 8 : 15;
-  int e = (int)(amax_bits >> 23) - 127 - EMAX + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
-  if (e < -126) e = -126;
-  if (amax_bits == 0) e = 0;
-  factor = __uint_as_float(amax_bits >= 0x7f800000u ? 0x7fc00000u : (uint32_t)(127 - e) << 23);
-  return e;
+  // exponent + 127 of the maximum, one more above 1.75 (a carry out of the mantissa), less EMAX; not under 2^-126
+  int e = (int)((amax_bits + 0x1fffffu) >> 23) - EMAX;
+  e = e < 1 ? 1 : e;
+  e = amax_bits == 0 ? 127 : e;
+  const bool finite = amax_bits < 0x7f800000u;
+  return {(uint8_t)e, finite, __uint_as_float((uint32_t)e << 23), __uint_as_float(finite ? (uint32_t)(254 - e) << 23 : 0x7fc00000u)};
 }
 
 template <int FMT> __device__ inline uint32_t pack4(float a, float b, float c, float d) {
@@ -116,8 +118,36 @@ template <> struct Eight<FT_F32> {
   __device__ float get(int j) const { return v[j]; }
 };
 
-template <int T, int FMT> __device__ inline uint2 quant8(const Eight<T>& x, float f) {
-  return make_uint2(pack4<FMT>(x.get(0) * f, x.get(1) * f, x.get(2) * f, x.get(3) * f), pack4<FMT>(x.get(4) * f, x.get(5) * f, x.get(6) * f, x.get(7) * f));
+// Four of eight values as 8-bit ones, x 2^-e.  16-bit values are converted in pairs by the instruction that scales on the way (it divides by
+// the power of two of `scale` exactly and rounds once); a block with a NaN or an infinity becomes NaN through its fp32 factor, or here.
+typedef short s16x2 __attribute__((ext_vector_type(2)));
+typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
+template <int T, int FMT> __device__ inline uint32_t cvt4(uint32_t lo, uint32_t hi, float scale) {
+  s16x2 w = {0, 0};
+  if constexpr (T == FT_F16 && FMT == F8_E4M3) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(h16x2, lo), scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f16(w, __builtin_bit_cast(h16x2, hi), scale, true);
+  } else if constexpr (T == FT_F16) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(w, __builtin_bit_cast(h16x2, lo), scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_bf8_f16(w, __builtin_bit_cast(h16x2, hi), scale, true);
+  } else if constexpr (FMT == F8_E4M3) {
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(b16x2, lo), scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(w, __builtin_bit_cast(b16x2, hi), scale, true);
+  } else {
+    w = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(w, __builtin_bit_cast(b16x2, lo), scale, false);
+    w = __builtin_amdgcn_cvt_scalef32_pk_bf8_bf16(w, __builtin_bit_cast(b16x2, hi), scale, true);
+  }
+  return __builtin_bit_cast(uint32_t, w);
+}
+template <int T, int FMT> __device__ inline uint2 quant8(const Eight<T>& x, const BlockScale& s) {
+  if constexpr (T == FT_F32) {
+    const float f = s.factor;
+    return make_uint2(pack4<FMT>(x.v[0] * f, x.v[1] * f, x.v[2] * f, x.v[3] * f), pack4<FMT>(x.v[4] * f, x.v[5] * f, x.v[6] * f, x.v[7] * f));
+  } else {
+    const i32x4 w = __builtin_bit_cast(i32x4, x.v);
+    const uint2 q = make_uint2(cvt4<T, FMT>(w[0], w[1], s.scale), cvt4<T, FMT>(w[2], w[3], s.scale));
+    return s.finite ? q : make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);       // (0x7f: a NaN of both formats)
+  }
 }
 
 // ------------------------------------------------------------------------------------------------------------ quantisers
@@ -131,10 +161,9 @@ __global__ __launch_bounds__(256) void k_fp8_quant(const void* __restrict__ x, i
     const int b = (int)(i - row * nb), k = b * 128 + sub * 8;
     Eight<T> v;
     v.load(x, row * ldx + k, K - k);
-    float f;
-    const int e = block_exp<FMT>(umax16(v.amax()), f);
-    *(uint2*)(q + row * ldq + k) = quant8<T, FMT>(v, f);
-    if (sub == 0) scale[row * lds + b] = (uint8_t)(e + 127);
+    const BlockScale bs = block_scale<FMT>(umax16(v.amax()));
+    *(uint2*)(q + row * ldq + k) = quant8<T, FMT>(v, bs);
+    if (sub == 0) scale[row * lds + b] = bs.byte;
     else if (sub < 4 && b == nb - 1 && nb + sub - 1 < (nb + 3) / 4 * 4) scale[row * lds + nb + sub - 1] = 127;   // the rest of the last word
   }
 }
@@ -176,13 +205,13 @@ __global__ __launch_bounds__(256) void k_fp8_quant_t(const void* __restrict__ x,
     uint32_t a = amax[0][c8 + j];
 #pragma unroll
     for (int w = 1; w < 4; ++w) a = amax[w][c8 + j] > a ? amax[w][c8 + j] : a;
-    float f;
-    const int e = block_exp<FMT>(a, f);
+    const BlockScale bs = block_scale<FMT>(a);
+    const float f = bs.factor;
     const uint32_t p = pack4<FMT>(v[0].get(j) * f, v[1].get(j) * f, v[2].get(j) * f, v[3].get(j) * f);
 #pragma unroll
     for (int i = 0; i < 4; ++i) tile[c8 + j][r0 + 32 * i] = (uint8_t)(p >> (8 * i));
     if (tid < 8 && c0 + c8 + j < C) {
-      scale[(c0 + c8 + j) * lds + b] = (uint8_t)(e + 127);
+      scale[(c0 + c8 + j) * lds + b] = bs.byte;
       if (b == nb - 1) for (int k = nb; k < (nb + 3) / 4 * 4; ++k) scale[(c0 + c8 + j) * lds + k] = 127;
     }
   }
@@ -200,7 +229,6 @@ template <int FA, int FB> __device__ inline f32x16 mfma8(i32x8 a, i32x8 b, f32x1
 }
 
 // two 8-bit values (the upper two of the word with HI) times a power of two, exact in bf16
-typedef __bf16 b16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 template <int FMT, bool HI> __device__ inline b16x2 widen2(uint32_t w, float s) {
@@ -211,6 +239,8 @@ template <int FMT> __device__ inline b16x8 widen8(uint32_t w0, uint32_t w1, floa
   const b16x2 a = widen2<FMT, false>(w0, s), b = widen2<FMT, true>(w0, s), c = widen2<FMT, false>(w1, s), d = widen2<FMT, true>(w1, s);
   return (b16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+
+__device__ inline float relu_nan(float v) { return __builtin_elementwise_maximum(v, 0.f); }     // a NaN stays one
 
 struct Fp8Out { void* y; int64_t ldy; int type, relu; };   // type: FT_*
 
@@ -229,13 +259,13 @@ __device__ inline void store_block(const Fp8Out& o, const f32x16& c0, const f32x
       f32x4 v = s ? (f32x4){c1[4 * g], c1[4 * g + 1], c1[4 * g + 2], c1[4 * g + 3]} : (f32x4){c0[4 * g], c0[4 * g + 1], c0[4 * g + 2], c0[4 * g + 3]};
       if (o.relu) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];       // (a NaN stays)
+        for (int j = 0; j < 4; ++j) v[j] = relu_nan(v[j]);
       }
       if constexpr (F32) *(f32x4*)(buf + r * 256 + (((8 * s + 2 * g + h) ^ (r & 15)) * 16)) = v;
       else {
         uint8_t* q = buf + r * 128 + (((4 * s + g) ^ (r & 7)) * 16) + 8 * h;
-        if (o.type == FT_F16) *(h16x4*)q = (h16x4){(h16)v[0], (h16)v[1], (h16)v[2], (h16)v[3]};
-        else *(b16x4*)q = (b16x4){(__bf16)v[0], (__bf16)v[1], (__bf16)v[2], (__bf16)v[3]};
+        if (o.type == FT_F16) *(h16x4*)q = __builtin_convertvector(v, h16x4);
+        else *(b16x4*)q = __builtin_convertvector(v, b16x4);
       }
     }
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -386,83 +416,131 @@ struct Fp8Linear {
 #define LIN_NKB 8
 static inline int lin_lds(int nkb) { return LIN_BM * nkb * 128 + 2 * 128 * 128 + LIN_BM * LIN_NKB; }
 
-template <int T, int FX, int FW>
-__global__ __launch_bounds__(256) void k_fp8_linear(Fp8Linear p) {
+template <int T, int FX>
+__global__ __launch_bounds__(256, 2) void k_fp8_linear(Fp8Linear p) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];
   uint8_t* xs = smem8;                                    // [64][nkb][128], pieces of 16 bytes turned by the row within each block
   uint8_t* ws = xs + LIN_BM * p.nkb * 128;                // [2][128][128]
   uint8_t* se = ws + 2 * 128 * 128;                       // [64][8] exponents + 127
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
-  const int wm = wave & 1, wn = wave >> 1;
+  const int wm = wave & 1, wn = wave >> 1, nkb = p.nkb;
   // blocks b and b + 8 run on the same XCD: the parts of a row tile go there and share its rows in that L2
   const int xcd = blockIdx.x & 7, jj = blockIdx.x >> 3;
   const int64_t m0 = ((int64_t)(jj / p.parts) * 8 + xcd) * LIN_BM;
   if (m0 >= p.M) return;
   const int t0 = (jj % p.parts) * p.per, t1 = min((p.N + 127) / 128, t0 + p.per);
-  const int steps = (t1 - t0) * p.nkb;
-  const int sub = lane >> 3, slot = lane & 7;
-  auto fetch = [&](int step) {
-    const int t = t0 + step / p.nkb, kb = step % p.nkb;
+  const int steps = (t1 - t0) * nkb;                      // >= 1
+  // The weights' tiles come through registers, two steps ahead of the one that is multiplied: a step's arithmetic is shorter than the way to
+  // L2.  The cursor (ft, fkb) runs over them; rows behind the last are clamped (their results are never stored).
+  i32x4 wa[4], wb[4];
+  const int wrow = tid >> 3, piece = tid & 7;             // rows wrow + 32 i of the tile, one 16-byte piece
+  const uint8_t* fp[4];
+  int ft = t0, fkb = 0;
+  auto aim = [&]() __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = (wave * 4 + i) * 8 + sub;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(p.w + (int64_t)min(t * 128 + row, p.N - 1) * p.ldw + kb * 128 + ((slot ^ (row & 7)) * 16)),
-                                       (__attribute__((address_space(3))) void*)(ws + (step & 1) * 16384 + (wave * 4 + i) * 1024), 16, 0, 0);
-    }
+    for (int i = 0; i < 4; ++i) fp[i] = p.w + (int64_t)min(ft * 128 + wrow + 32 * i, p.N - 1) * p.ldw + piece * 16;
   };
-  if (steps > 0) fetch(0);
+  auto fetch = [&](i32x4 (&w4)[4]) __attribute__((always_inline)) {
+    if (ft >= t1) return;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { w4[i] = *(const i32x4*)fp[i]; fp[i] += 128; }
+    if (++fkb == nkb) { fkb = 0; ++ft; aim(); }
+  };
+  const int put = wrow * 128 + ((piece ^ (wrow & 7)) * 16);
+  auto stash = [&](int half, const i32x4 (&w4)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(i32x4*)(ws + half * 16384 + put + i * 4096) = w4[i];
+  };
+  aim();
+  fetch(wa);
+  fetch(wb);
+  // four lanes hold a block of a row, pieces l, l + 4, ... of eight values each: its maximum takes two exchanges, its power of two is worked
+  // out once for 32 values of a lane
   {
-    const int g = tid >> 4, s16 = tid & 15;               // 16 lanes a block of 128, 16 rows at a time
-    for (int b = 0; b < p.nkb; ++b) {
-      Eight<T> v[4];
+    const int row = tid >> 2, l = tid & 3;
+    const int64_t at = min(m0 + row, p.M - 1) * p.ldx;
+    uint8_t* dst = xs + row * nkb * 128;
+    for (int b0 = 0; b0 < nkb; b0 += 4) {
+      Eight<T> v[4][4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) { const int k = b * 128 + s16 * 8; v[i].load(p.x, min(m0 + 16 * i + g, p.M - 1) * p.ldx + k, p.K - k); }
+      for (int b = 0; b < 4; ++b)
+        if (b0 + b < nkb) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int row = 16 * i + g;
-        float f;
-        const int e = block_exp<FX>(umax16(v[i].amax()), f);
-        *(uint2*)(xs + (row * p.nkb + b) * 128 + (((s16 >> 1) ^ (row & 7)) * 16) + (s16 & 1) * 8) = quant8<T, FX>(v[i], f);
-        if (s16 == 0) se[row * LIN_NKB + b] = (uint8_t)(e + 127);
-      }
+          for (int j = 0; j < 4; ++j) { const int k = (b0 + b) * 128 + (4 * j + l) * 8; v[b][j].load(p.x, at + k, p.K - k); }
+        }
+#pragma unroll
+      for (int b = 0; b < 4; ++b)
+        if (b0 + b < nkb) {
+          uint32_t m = 0;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { const uint32_t a = v[b][j].amax(); m = a > m ? a : m; }
+          const BlockScale bs = block_scale<FX>(dpp_umax<0x4E>(dpp_umax<0xB1>(m)));
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            *(uint2*)(dst + (b0 + b) * 128 + (((2 * j + (l >> 1)) ^ (row & 7)) * 16) + (l & 1) * 8) = quant8<T, FX>(v[b][j], bs);
+          if (l == 0) se[row * LIN_NKB + b0 + b] = bs.byte;
+        }
     }
   }
+  stash(0, wa);
+  fetch(wa);
+  // the weights' exponents, four blocks to a word, a group of four blocks ahead
+  const uint8_t* sp[2];
+  uint32_t sw_now[2] = {0, 0}, sw_next[2];
+  auto aim_scales = [&](int t) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) { sp[i] = p.sw + (int64_t)min(t * 128 + wn * 64 + i * 32 + r, p.N - 1) * p.ldsw; sw_next[i] = *(const uint32_t*)sp[i]; }
+  };
+  aim_scales(t0);
   __syncthreads();
   f32x16 acc[2];
   const int xrow = wm * 32 + r;
-  for (int step = 0; step < steps; ++step) {
-    const int t = t0 + step / p.nkb, kb = step % p.nkb;
-    if (step + 1 < steps) fetch(step + 1);
+  const uint8_t* xr0 = xs + xrow * nkb * 128;
+  const uint8_t* wr0 = ws + (wn * 64 + r) * 128;
+  int off[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) off[c] = ((4 * h + c) ^ (r & 7)) * 16;
+  int t = t0, kb = 0;
+  auto one = [&](int half, i32x4 (&next)[4]) __attribute__((always_inline)) {            // `next` holds the tile of the next step
     if (kb == 0) {
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
     }
-    int sb[2];
+    if ((kb & 3) == 0) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) sb[i] = p.sw[(int64_t)min(t * 128 + wn * 64 + i * 32 + r, p.N - 1) * p.ldsw + kb];
+      for (int i = 0; i < 2; ++i) sw_now[i] = sw_next[i];
+      if (kb + 4 < nkb) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) sw_next[i] = *(const uint32_t*)(sp[i] + kb + 4);
+      } else aim_scales(t + 1);
+    }
     const int sa = se[xrow * LIN_NKB + kb];
-    const uint8_t* xr = xs + (xrow * p.nkb + kb) * 128;
-    const uint8_t* wt = ws + (step & 1) * 16384;
+    const uint8_t *xr = xr0 + kb * 128, *wr = wr0 + half * 16384;
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const int c0 = 4 * h + 2 * ks, o0 = (c0 ^ (r & 7)) * 16, o1 = ((c0 + 1) ^ (r & 7)) * 16;
-      const i32x8 fx = __builtin_shufflevector(*(const i32x4*)(xr + o0), *(const i32x4*)(xr + o1), 0, 1, 2, 3, 4, 5, 6, 7);
+      const i32x8 fx = __builtin_shufflevector(*(const i32x4*)(xr + off[2 * ks]), *(const i32x4*)(xr + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint8_t* wr = wt + (wn * 64 + i * 32 + r) * 128;
-        const i32x8 fw = __builtin_shufflevector(*(const i32x4*)(wr + o0), *(const i32x4*)(wr + o1), 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[i] = mfma8<FW, FX>(fw, fx, acc[i], sb[i], sa);
+        const i32x8 fw = __builtin_shufflevector(*(const i32x4*)(wr + i * 4096 + off[2 * ks]), *(const i32x4*)(wr + i * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+        acc[i] = mfma8<F8_E4M3, FX>(fw, fx, acc[i], (int)sw_now[i], sa);
       }
     }
-    __syncthreads();            // the tile has been read, the next one has landed
-    if (kb == p.nkb - 1) {
-      // the next tile has landed in the other half: this one's is free for the result
-      uint8_t* buf = ws + (step & 1) * 16384 + wave * 4096;
-      store_block<false>(p.o, acc[0], acc[1], buf, m0 + wm * 32, p.M, t * 128 + wn * 64, p.N, lane);
-      __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sw_now[i] >>= 8;
+    if (++kb == nkb) {
+      __syncthreads();          // every wave is done with this half of the tiles: it takes the result's turn
+      store_block<false>(p.o, acc[0], acc[1], ws + half * 16384 + wave * 4096, m0 + wm * 32, p.M, t * 128 + wn * 64, p.N, lane);
+      kb = 0; ++t;
     }
+    stash(half ^ 1, next);
+    fetch(next);
+    __syncthreads();
+  };
+  for (int step = 0; step < steps; step += 2) {
+    one(0, wb);
+    if (step + 1 < steps) one(1, wa);
   }
 }
 
@@ -472,7 +550,7 @@ __global__ __launch_bounds__(256) void k_fp8_join(const float* __restrict__ slab
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
     float s = 0.f;
     for (int k = 0; k < splits; ++k) s += slabs[k * n + i];
-    if (o.relu) s = s < 0.f ? 0.f : s;
+    if (o.relu) s = relu_nan(s);
     const int64_t at = i / N * o.ldy + i % N;
     if (o.type == FT_F32) ((float*)o.y)[at] = s;
     else if (o.type == FT_F16) ((h16*)o.y)[at] = (h16)s;
@@ -575,26 +653,23 @@ extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t
   return 0;
 }
 
-// ---- x W^T for x as it is.  Up to 1024 columns and 16-bit results: the one-launch kernel; otherwise blocks of x in the workspace, then the product.
-static bool lin_fused(int64_t K, int y_type) { return ceil128(K) / 128 <= LIN_NKB && y_type != FT_F32; }
+// ---- x W^T for x as it is.  Up to 1024 columns, 16-bit x and y, e4m3 weights: the one-launch kernel; otherwise blocks of x in the workspace,
+// then the product.
+static bool lin_fused(int64_t K, int x_type, int y_type, int fmt_w) { return ceil128(K) / 128 <= LIN_NKB && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3; }
 static inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
-extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t y_type) {
-  if (M <= 0 || N <= 0 || K <= 0 || lin_fused(K, y_type)) return 0;
+extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t x_type, int32_t y_type, int32_t fmt_w) {
+  if (M <= 0 || N <= 0 || K <= 0 || lin_fused(K, x_type, y_type, fmt_w)) return 0;
   const int64_t nb = ceil128(K) / 128;
   return M * nb * 128 + up16(M * ((nb + 3) / 4 * 4)) + aln_fp8_nt_ws_bytes(M, N, K);
 }
-template <int T, int FX, int FW> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
-  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_linear<T, FX, FW>, hipFuncAttributeMaxDynamicSharedMemorySize, lin_lds(LIN_NKB));
+template <int T, int FX> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
+  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_linear<T, FX>, hipFuncAttributeMaxDynamicSharedMemorySize, lin_lds(LIN_NKB));
   ALN_REQUIRE(big == hipSuccess, "fp8_linear: %s", hipGetErrorString(big));
   const int64_t g = ((p.M + LIN_BM - 1) / LIN_BM + 7) / 8 * 8 * p.parts;
   ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_linear: %lld x %d results are too many for one launch", (long long)p.M, p.N);
-  hipLaunchKernelGGL((k_fp8_linear<T, FX, FW>), dim3((uint32_t)g), dim3(256), lin_lds(p.nkb), st, p);
+  hipLaunchKernelGGL((k_fp8_linear<T, FX>), dim3((uint32_t)g), dim3(256), lin_lds(p.nkb), st, p);
   ALN_CHECK_LAUNCH("fp8_linear");
   return 0;
-}
-template <int T> static int lin_fmt(int fx, int fw, const Fp8Linear& p, hipStream_t st) {
-  return fx == F8_E4M3 ? (fw == F8_E4M3 ? lin_launch<T, F8_E4M3, F8_E4M3>(p, st) : lin_launch<T, F8_E4M3, F8_E5M2>(p, st))
-                       : (fw == F8_E4M3 ? lin_launch<T, F8_E5M2, F8_E4M3>(p, st) : lin_launch<T, F8_E5M2, F8_E5M2>(p, st));
 }
 extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, const void* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, int32_t fmt_w,
                               int64_t M, int32_t N, int32_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws, int64_t ws_bytes, void* stream) {
@@ -604,10 +679,10 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
   if (M == 0) return 0;
   ALN_REQUIRE(blocks_ok(w, ldw, sw, ldsw, K), FP8_BAD_BLOCKS, "fp8_linear");
   ALN_REQUIRE(x && ((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0 && y && ((uintptr_t)y & (y_type == FT_F32 ? 3 : 1)) == 0, "fp8_linear: x or y is NULL or not aligned to its type");
-  const int64_t need = aln_fp8_linear_ws_bytes(M, N, K, y_type);
+  const int64_t need = aln_fp8_linear_ws_bytes(M, N, K, x_type, y_type, fmt_w);
   ALN_REQUIRE(ws_bytes >= need && (need == 0 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_linear: the workspace needs %lld bytes, aligned to 16", (long long)need);
   const int nkb = (int)(ceil128(K) / 128);
-  if (!lin_fused(K, y_type)) {
+  if (!lin_fused(K, x_type, y_type, fmt_w)) {
     uint8_t* q = (uint8_t*)ws, *sc = q + M * nkb * 128, *rest = sc + up16(M * ((nkb + 3) / 4 * 4));
     const int rc = aln_fp8_quantize(x, x_type, ldx, M, K, fmt_x, q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, stream);
     if (rc) return rc;
@@ -621,5 +696,6 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
   const int per = (nt + parts - 1) / parts;
   const Fp8Linear p{x, ldx, (const uint8_t*)w, ldw, sw, ldsw, M, N, K, nkb, (nt + per - 1) / per, per, Fp8Out{y, ldy, y_type, relu}};
   hipStream_t st = (hipStream_t)stream;
-  return x_type == FT_F16 ? lin_fmt<FT_F16>(fmt_x, fmt_w, p, st) : x_type == FT_BF16 ? lin_fmt<FT_BF16>(fmt_x, fmt_w, p, st) : lin_fmt<FT_F32>(fmt_x, fmt_w, p, st);
+  return x_type == FT_F16 ? (fmt_x == F8_E4M3 ? lin_launch<FT_F16, F8_E4M3>(p, st) : lin_launch<FT_F16, F8_E5M2>(p, st))
+                          : (fmt_x == F8_E4M3 ? lin_launch<FT_BF16, F8_E4M3>(p, st) : lin_launch<FT_BF16, F8_E5M2>(p, st));
 }

@@ -145,7 +145,7 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
     _need(n >= 1, 'linear: the weight has no rows')
     with _on(rows, weight.q):
         y = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
-        nbytes = H.lib().aln_fp8_linear_ws_bytes(m, n, k, TYPES[out_dtype])
+        nbytes = H.lib().aln_fp8_linear_ws_bytes(m, n, k, TYPES[x.dtype], TYPES[out_dtype], FORMATS[weight.fmt][0])
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         H.call('aln_fp8_linear', _p(rows), TYPES[x.dtype], _pitch(rows), FORMATS[fmt][0], _p(weight.q), weight.q.shape[1], _p(weight.scale),
                weight.scale.shape[1], FORMATS[weight.fmt][0], m, n, k, _p(y), n, TYPES[out_dtype], int(bool(relu)), _p(ws) if nbytes else None, nbytes,

@@ -129,7 +129,7 @@ _SIGS = {
     'aln_fp8_quantize_t': (i32, [vp, i32, i64, i64, i32, i32, vp, i64, vp, i64, vp]),
     'aln_fp8_nt_ws_bytes': (i64, [i64, i32, i64]),
     'aln_fp8_nt': (i32, [vp, i64, vp, i64, i32, vp, i64, vp, i64, i32, i64, i32, i64, vp, i64, i32, i32, vp, i64, vp]),
-    'aln_fp8_linear_ws_bytes': (i64, [i64, i32, i32, i32]),
+    'aln_fp8_linear_ws_bytes': (i64, [i64, i32, i32, i32, i32, i32]),
     'aln_fp8_linear': (i32, [vp, i32, i64, i32, vp, i64, vp, i64, i32, i64, i32, i32, vp, i64, i32, i32, vp, i64, vp]),
     'aln_grad_clip_ws_bytes': (i64, [i32]),
     'aln_grad_clip': (i32, [i32, vp, vp, vp, vp, f32, i32, vp, vp, vp, vp, i64, vp]),

@@ -468,9 +468,9 @@ int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t ldsa, int3
                int64_t ws_bytes, void* stream);
 
 /* y [M, N] = x W^T for x [M, K] as it is (row pitch ldx): its rows are cut into blocks of fmt_x on the way -- the same result as
- * aln_fp8_quantize + aln_fp8_nt up to the order of the fp32 additions.  ws: aln_fp8_linear_ws_bytes(M, N, K, y_type) bytes, 16-byte aligned
+ * aln_fp8_quantize + aln_fp8_nt up to the order of the fp32 additions.  ws: aln_fp8_linear_ws_bytes(same sizes and types) bytes, 16-byte aligned
  * (0: may be NULL). */
-int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t y_type);
+int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t x_type, int32_t y_type, int32_t fmt_w);
 int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, const void* w, int64_t ldw, const uint8_t* sw, int64_t ldsw,
                    int32_t fmt_w, int64_t M, int32_t N, int32_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws,
                    int64_t ws_bytes, void* stream);
