@@ -544,6 +544,157 @@ __global__ __launch_bounds__(256, 2) void k_fp8_linear(Fp8Linear p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------------ weight gradients
+// dW = G^T X over the rows of g and x, both cut into blocks of 128 ROWS per column on the way.  The result is fp32 and the sum long, so the
+// 8-bit values go back to bf16 (exactly) for the bf16 matrix instruction.  A block of 8 waves owns 64 NI x 256 results and a range of
+// 128-row steps.  Per step every wave turns strips of 128 rows x 32 columns round: a lane holds 8 rows x 8 columns (rows rg, rg + 16, ...: a
+// load instruction reads 64 bytes of 16 rows), pairs up its rows (v_perm), the column's maximum crosses the 16 lanes of a DPP row, and each
+// column leaves as 128 bytes of 8-bit values.  Both operands carry the same order of the rows, whatever it is.
+// Two LDS buffers: while a step is multiplied the strips of the next one are cut into blocks, and the loads of the strip after that are in flight.
+struct Fp8TN {
+  const void* g; int64_t ldg; const void* x; int64_t ldx;
+  int64_t M; int N, K;
+  int tn, tk, per;                // tiles of the result, steps of a part
+  float* y;                       // [parts][N][K]
+};
+
+__device__ inline uint32_t pk_max16(uint32_t a, uint32_t b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+template <int CTRL> __device__ inline uint32_t dpp_pk_max16(uint32_t v) {
+  return pk_max16(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false));
+}
+
+// one strip: v[i] = eight columns of row i * 16 + rg; tile: [32 columns][128 bytes], scale: their powers of two
+template <int T, int FMT> __device__ inline void tn_quant(const u16x8 (&v)[8], uint8_t* tile, float* scale, int lane) {
+  const int rg = lane & 15, c8 = (lane >> 4) * 8;
+  // maxima of the eight columns, two to a word
+  uint32_t m[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    m[k] = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[k] = pk_max16(m[k], __builtin_bit_cast(i32x4, v[i])[k] & 0x7fff7fff);
+    m[k] = dpp_pk_max16<0xB1>(m[k]);
+    m[k] = dpp_pk_max16<0x4E>(m[k]);
+    m[k] = dpp_pk_max16<0x141>(m[k]);
+    m[k] = dpp_pk_max16<0x140>(m[k]);
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const uint32_t a = (j & 1) ? m[j / 2] >> 16 : m[j / 2] & 0xffffu;
+    const BlockScale bs = block_scale<FMT>(T == FT_F16 ? __float_as_uint((float)__builtin_bit_cast(h16, (uint16_t)a)) : a << 16);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)        // column j of two rows in one word
+      w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(i32x4, v[2 * i + 1])[j / 2], __builtin_bit_cast(i32x4, v[2 * i])[j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
+    uint2 q = make_uint2(cvt4<T, FMT>(w[0], w[1], bs.scale), cvt4<T, FMT>(w[2], w[3], bs.scale));
+    if (!bs.finite) q = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
+    const int c = c8 + j;
+    *(uint2*)(tile + c * 128 + (((rg >> 1) ^ (c & 7)) * 16) + (rg & 1) * 8) = q;
+    if (rg == j) scale[c] = bs.scale;
+  }
+}
+
+template <int T, int FG, int NI>
+__global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
+  constexpr int TN = 64 * NI, TK = 256, COLS = TN + TK, STRIPS = COLS / 32;      // 8 < STRIPS <= 16
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];     // [2][COLS][128], then [2][COLS] powers of two
+  float* scales = (float*)(smem8 + 2 * COLS * 128);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  const int wn = wave & 1, wk = wave >> 1;                // waves: 2 along n (32 NI columns each), 4 along k (64 each)
+  // blocks b and b + 8 run on the same XCD: the tiles of a part go there back to back and share its rows in that L2
+  const int tiles = p.tn * p.tk, xcd = blockIdx.x & 7, jj = blockIdx.x >> 3, part = (jj / tiles) * 8 + xcd, tile = jj % tiles;
+  const int64_t nsteps = (p.M + 127) / 128, s0 = (int64_t)part * p.per, s1 = s0 + p.per < nsteps ? s0 + p.per : nsteps;
+  if (s0 >= nsteps) return;
+  const int n0 = tile / p.tk * TN, k0 = tile % p.tk * TK;
+  f32x16 acc[NI][2];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  u16x8 v[8];                                             // one strip on its way
+  const int rg = lane & 15, c8 = (lane >> 4) * 8;
+  auto load = [&](int64_t step, int strip) __attribute__((always_inline)) {
+    if (step >= s1 || strip >= STRIPS) return;
+    const bool isg = strip < TN / 32;
+    const uint16_t* base = (const uint16_t*)(isg ? p.g : p.x);
+    const int64_t ld = isg ? p.ldg : p.ldx;
+    const int C = isg ? p.N : p.K, col = (isg ? n0 + strip * 32 : k0 + (strip - TN / 32) * 32) + c8;
+    const int64_t row = step * 128 + rg;
+    const uint16_t* at = base + row * ld + col;
+    if (step * 128 + 128 <= p.M && col - c8 + 32 <= C) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) __builtin_memcpy(&v[i], at + i * 16 * ld, 16);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) { Eight<T> e; e.load(at + i * 16 * ld, 0, row + i * 16 < p.M ? C - col : 0); v[i] = e.v; }
+    }
+  };
+  auto cut = [&](int64_t step, int strip) __attribute__((always_inline)) {
+    if (step >= s1 || strip >= STRIPS) return;
+    const int buf = (int)(step - s0) & 1;
+    uint8_t* t = smem8 + (buf * COLS + strip * 32) * 128;
+    float* sc = scales + buf * COLS + strip * 32;
+    if (strip < TN / 32) tn_quant<T, FG>(v, t, sc, lane);
+    else tn_quant<T, F8_E4M3>(v, t, sc, lane);
+  };
+  load(s0, wave);
+  cut(s0, wave);
+  load(s0, wave + 8);
+  cut(s0, wave + 8);
+  load(s0 + 1, wave);
+  __syncthreads();
+  for (int64_t s = s0; s < s1; ++s) {
+    const int buf = (int)(s - s0) & 1;
+    const uint8_t* gt = smem8 + (buf * COLS + wn * 32 * NI + r) * 128;
+    const uint8_t* xt = smem8 + (buf * COLS + TN + wk * 64 + r) * 128;
+    const float* sc = scales + buf * COLS;
+    float sg[NI], sx[2];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sg[i] = sc[wn * 32 * NI + 32 * i + r];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) sx[j] = sc[TN + wk * 64 + 32 * j + r];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int off = ((4 * h + c) ^ (r & 7)) * 16;
+      i32x4 fg[NI], fx[2];
+#pragma unroll
+      for (int i = 0; i < NI; ++i) fg[i] = *(const i32x4*)(gt + i * 4096 + off);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) fx[j] = *(const i32x4*)(xt + j * 4096 + off);
+#pragma unroll
+      for (int q = 0; q < 2; ++q) {
+        b16x8 bx[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) bx[j] = widen8<F8_E4M3>(fx[j][2 * q], fx[j][2 * q + 1], sx[j]);
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const b16x8 bg = widen8<FG>(fg[i][2 * q], fg[i][2 * q + 1], sg[i]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bg, bx[j], acc[i][j], 0, 0, 0);
+        }
+      }
+      if (c == 1) { cut(s + 1, wave); load(s + 1, wave + 8); }
+      if (c == 3) { cut(s + 1, wave + 8); load(s + 2, wave); }
+    }
+    __syncthreads();            // this step's tile has been read, the next one is written
+  }
+  float* y = p.y + (int64_t)part * p.N * p.K;
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int n = n0 + wn * 32 * NI + 32 * i + 8 * (e / 4) + 4 * h + e % 4, k = k0 + wk * 64 + 32 * j + r;
+        if (n < p.N && k < p.K) y[(int64_t)n * p.K + k] = acc[i][j][e];
+      }
+}
+
 // the slabs of a split contraction, added in their order and rounded once
 __global__ __launch_bounds__(256) void k_fp8_join(const float* __restrict__ slabs, int splits, int64_t M, int N, Fp8Out o) {
   const int64_t n = M * N;
@@ -698,4 +849,66 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
   hipStream_t st = (hipStream_t)stream;
   return x_type == FT_F16 ? (fmt_x == F8_E4M3 ? lin_launch<FT_F16, F8_E4M3>(p, st) : lin_launch<FT_F16, F8_E5M2>(p, st))
                           : (fmt_x == F8_E4M3 ? lin_launch<FT_BF16, F8_E4M3>(p, st) : lin_launch<FT_BF16, F8_E5M2>(p, st));
+}
+
+// ---- dW [N, K] (fp32, contiguous) = G^T X over M rows.  16-bit g and x of one type: the one-launch kernel (and the addition of its parts);
+// otherwise both transposed into blocks in the workspace, then the product.
+static bool tn_fused(int g_type, int x_type) { return g_type == x_type && g_type != FT_F32; }
+struct TnPlan { int ni, tn, tk, parts, per; };
+static TnPlan tn_plan(int64_t M, int N, int K) {
+  TnPlan t;
+  t.ni = N > 128 ? 4 : 2;
+  t.tn = (N + 64 * t.ni - 1) / (64 * t.ni); t.tk = (K + 255) / 256;
+  const int64_t tiles = (int64_t)t.tn * t.tk, steps = (M + 127) / 128;
+  int64_t parts = tiles >= 256 ? 1 : 256 / tiles;         // one block per CU
+  if (parts > (steps + 3) / 4) parts = (steps + 3) / 4;   // four steps at least
+  t.per = (int)((steps + parts - 1) / parts);
+  t.parts = (int)((steps + t.per - 1) / t.per);
+  return t;
+}
+extern "C" int64_t aln_fp8_grad_weight_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t g_type, int32_t x_type) {
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  if (tn_fused(g_type, x_type)) { const TnPlan t = tn_plan(M, N, K); return t.parts > 1 ? (int64_t)t.parts * N * K * 4 : 0; }
+  const int64_t nb = ceil128(M) / 128, per_row = nb * 128 + (nb + 3) / 4 * 4;
+  return up16(((int64_t)N + K) * per_row) + 16 * 4 + aln_fp8_nt_ws_bytes(N, K, M);
+}
+template <int T, int FG, int NI> static int tn_launch(const Fp8TN& p, int parts, hipStream_t st) {
+  constexpr int COLS = 64 * NI + 256, LDS = 2 * COLS * 132;
+  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  ALN_REQUIRE(big == hipSuccess, "fp8_grad_weight: %s", hipGetErrorString(big));
+  const int64_t g = (int64_t)(parts + 7) / 8 * 8 * p.tn * p.tk;
+  ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_grad_weight: %d x %d results are too many for one launch", p.N, p.K);
+  hipLaunchKernelGGL((k_fp8_tn<T, FG, NI>), dim3((uint32_t)g), dim3(512), LDS, st, p);
+  ALN_CHECK_LAUNCH("fp8_grad_weight");
+  return 0;
+}
+template <int T> static int tn_pick(const Fp8TN& p, const TnPlan& t, int fmt_g, hipStream_t st) {
+  if (fmt_g == F8_E4M3) return t.ni == 4 ? tn_launch<T, F8_E4M3, 4>(p, t.parts, st) : tn_launch<T, F8_E4M3, 2>(p, t.parts, st);
+  return t.ni == 4 ? tn_launch<T, F8_E5M2, 4>(p, t.parts, st) : tn_launch<T, F8_E5M2, 2>(p, t.parts, st);
+}
+extern "C" int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, int32_t fmt_g, const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t N, int32_t K,
+                                   float* dw, void* ws, int64_t ws_bytes, void* stream) {
+  ALN_REQUIRE(is_ft(g_type) && is_ft(x_type) && is_f8(fmt_g), "fp8_grad_weight: unknown type %d, %d or format %d", g_type, x_type, fmt_g);
+  ALN_REQUIRE(M >= 1 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldg >= 0 && ldx >= 0, "fp8_grad_weight: sizes %lld x %d x %d, pitches %lld, %lld", (long long)M, N, K,
+              (long long)ldg, (long long)ldx);
+  ALN_REQUIRE(g && ((uintptr_t)g & (g_type == FT_F32 ? 3 : 1)) == 0 && x && ((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0 && dw && ((uintptr_t)dw & 3) == 0,
+              "fp8_grad_weight: g, x or dw is NULL or not aligned to its type");
+  const int64_t need = aln_fp8_grad_weight_ws_bytes(M, N, K, g_type, x_type);
+  ALN_REQUIRE(ws_bytes >= need && (need == 0 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_grad_weight: the workspace needs %lld bytes, aligned to 16", (long long)need);
+  hipStream_t st = (hipStream_t)stream;
+  if (!tn_fused(g_type, x_type)) {
+    const int64_t nb = ceil128(M) / 128, ld = nb * 128, lds = (nb + 3) / 4 * 4;
+    uint8_t *qg = (uint8_t*)ws, *qx = qg + N * ld, *sg = qx + K * ld, *sx = sg + up16(N * lds), *rest = sx + up16(K * lds);
+    int rc = aln_fp8_quantize_t(g, g_type, ldg, M, N, fmt_g, qg, ld, sg, lds, stream);
+    if (rc == 0) rc = aln_fp8_quantize_t(x, x_type, ldx, M, K, F8_E4M3, qx, ld, sx, lds, stream);
+    if (rc) return rc;
+    return aln_fp8_nt(qg, ld, sg, lds, fmt_g, qx, ld, sx, lds, F8_E4M3, N, K, M, dw, K, FT_F32, 0, rest, ws_bytes - (rest - qg), stream);
+  }
+  const TnPlan t = tn_plan(M, N, K);
+  const Fp8TN p{g, ldg, x, ldx, M, N, K, t.tn, t.tk, t.per, t.parts > 1 ? (float*)ws : dw};
+  const int rc = g_type == FT_F16 ? tn_pick<FT_F16>(p, t, fmt_g, st) : tn_pick<FT_BF16>(p, t, fmt_g, st);
+  if (rc || t.parts == 1) return rc;
+  hipLaunchKernelGGL(k_fp8_join, dim3(aln_grid_for((int64_t)N * K, 256, 2048)), dim3(256), 0, st, (const float*)ws, t.parts, (int64_t)N, K, Fp8Out{dw, K, FT_F32, 0});
+  ALN_CHECK_LAUNCH("fp8_grad_weight");
+  return 0;
 }

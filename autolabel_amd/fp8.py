@@ -170,10 +170,14 @@ def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True)
         dx = linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt).reshape(x.shape)
     if need_dw:
         with _on(gr, xr):
-            if gr.shape[0] == 0:
-                dw = torch.zeros(gr.shape[1], xr.shape[1], device=x.device)
-            else:
-                dw = matmul(quantize(gr, grad_fmt, transpose=True), quantize(xr, transpose=True), torch.float32)
+            (m, n), k = gr.shape, xr.shape[1]
+            if m == 0:
+                return dx, torch.zeros(n, k, device=x.device)
+            dw = torch.empty(n, k, device=x.device)
+            nbytes = H.lib().aln_fp8_grad_weight_ws_bytes(m, n, k, TYPES[g.dtype], TYPES[x.dtype])
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+            H.call('aln_fp8_grad_weight', _p(gr), TYPES[g.dtype], _pitch(gr), FORMATS[grad_fmt][0], _p(xr), TYPES[x.dtype], _pitch(xr), m, n, k,
+                   _p(dw), _p(ws) if nbytes else None, nbytes, H.stream())
     return dx, dw
 
 

@@ -131,6 +131,8 @@ _SIGS = {
     'aln_fp8_nt': (i32, [vp, i64, vp, i64, i32, vp, i64, vp, i64, i32, i64, i32, i64, vp, i64, i32, i32, vp, i64, vp]),
     'aln_fp8_linear_ws_bytes': (i64, [i64, i32, i32, i32, i32, i32]),
     'aln_fp8_linear': (i32, [vp, i32, i64, i32, vp, i64, vp, i64, i32, i64, i32, i32, vp, i64, i32, i32, vp, i64, vp]),
+    'aln_fp8_grad_weight_ws_bytes': (i64, [i64, i32, i32, i32, i32]),
+    'aln_fp8_grad_weight': (i32, [vp, i32, i64, i32, vp, i32, i64, i64, i32, i32, vp, vp, i64, vp]),
     'aln_grad_clip_ws_bytes': (i64, [i32]),
     'aln_grad_clip': (i32, [i32, vp, vp, vp, vp, f32, i32, vp, vp, vp, vp, i64, vp]),
     'aln_lzf_decompress': (i64, [C.c_char_p, C.c_size_t, C.c_char_p, C.c_size_t]),
