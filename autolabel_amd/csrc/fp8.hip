@@ -567,7 +567,9 @@ template <int CTRL> __device__ inline uint32_t dpp_pk_max16(uint32_t v) {
 }
 
 // one strip: v[i] = eight columns of row i * 16 + rg; tile: [32 columns][128 bytes], scale: their powers of two
-template <int T, int FMT> __device__ inline void tn_quant(const u16x8 (&v)[8], uint8_t* tile, float* scale, int lane) {
+template <int T, int FMT> __device__ inline void tn_quant(u16x8 (&v)[8], uint8_t* tile, float* scale, int lane) {
+  constexpr int EMAX = FMT == F8_E4M3 ? 8 : 15;
+  constexpr uint32_t INF = T == FT_F16 ? 0x7c00u : 0x7f80u;
   const int rg = lane & 15, c8 = (lane >> 4) * 8;
   // maxima of the eight columns, two to a word
   uint32_t m[4];
@@ -581,20 +583,30 @@ template <int T, int FMT> __device__ inline void tn_quant(const u16x8 (&v)[8], u
     m[k] = dpp_pk_max16<0x141>(m[k]);
     m[k] = dpp_pk_max16<0x140>(m[k]);
   }
+  const uint32_t most = pk_max16(pk_max16(m[0], m[1]), pk_max16(m[2], m[3]));
+  if (__any((most >> 16) >= INF || (most & 0xffffu) >= INF)) {      // a column with a NaN or an infinity becomes NaN throughout
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (((m[j / 2] >> (16 * (j & 1))) & 0xffffu) >= INF) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i][j] = 0x7fff;
+      }
+  }
+  float s[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const uint32_t a = (j & 1) ? m[j / 2] >> 16 : m[j / 2] & 0xffffu;
-    const BlockScale bs = block_scale<FMT>(T == FT_F16 ? __float_as_uint((float)__builtin_bit_cast(h16, (uint16_t)a)) : a << 16);
+    const uint32_t bits = T == FT_F16 ? __float_as_uint((float)__builtin_bit_cast(h16, (uint16_t)a)) : a << 16;
+    // block_scale's power of two (a column of zeros may have any)
+    const int e = (int)(bits + 0x1fffffu) - (EMAX << 23);
+    s[j] = __uint_as_float((uint32_t)(e < 1 << 23 ? 1 << 23 : e) & 0x7f800000u);
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i)        // column j of two rows in one word
       w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(i32x4, v[2 * i + 1])[j / 2], __builtin_bit_cast(i32x4, v[2 * i])[j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
-    uint2 q = make_uint2(cvt4<T, FMT>(w[0], w[1], bs.scale), cvt4<T, FMT>(w[2], w[3], bs.scale));
-    if (!bs.finite) q = make_uint2(0x7f7f7f7fu, 0x7f7f7f7fu);
-    const int c = c8 + j;
-    *(uint2*)(tile + c * 128 + (((rg >> 1) ^ (c & 7)) * 16) + (rg & 1) * 8) = q;
-    if (rg == j) scale[c] = bs.scale;
+    *(uint2*)(tile + (c8 + j) * 128 + ((((rg >> 1) ^ j) * 16) | ((rg & 1) * 8))) = make_uint2(cvt4<T, FMT>(w[0], w[1], s[j]), cvt4<T, FMT>(w[2], w[3], s[j]));
   }
+  if (rg == 0) { *(f32x4*)(scale + c8) = (f32x4){s[0], s[1], s[2], s[3]}; *(f32x4*)(scale + c8 + 4) = (f32x4){s[4], s[5], s[6], s[7]}; }
 }
 
 template <int T, int FG, int NI>
@@ -602,6 +614,7 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
   constexpr int TN = 64 * NI, TK = 256, COLS = TN + TK, STRIPS = COLS / 32;      // 8 < STRIPS <= 16
   extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];     // [2][COLS][128], then [2][COLS] powers of two
   float* scales = (float*)(smem8 + 2 * COLS * 128);
+  uint16_t* spare = (uint16_t*)(smem8 + 2 * COLS * 132);              // [512][8]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
   const int wn = wave & 1, wk = wave >> 1;                // waves: 2 along n (32 NI columns each), 4 along k (64 each)
   // blocks b and b + 8 run on the same XCD: the tiles of a part go there back to back and share its rows in that L2
@@ -617,21 +630,34 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
   u16x8 v[8];                                             // one strip on its way
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = (u16x8)(uint16_t)0;
   const int rg = lane & 15, c8 = (lane >> 4) * 8;
   auto load = [&](int64_t step, int strip) __attribute__((always_inline)) {
     if (step >= s1 || strip >= STRIPS) return;
+    // a uniform base and a 32-bit offset of the lane: no 64-bit arithmetic per lane
     const bool isg = strip < TN / 32;
-    const uint16_t* base = (const uint16_t*)(isg ? p.g : p.x);
     const int64_t ld = isg ? p.ldg : p.ldx;
-    const int C = isg ? p.N : p.K, col = (isg ? n0 + strip * 32 : k0 + (strip - TN / 32) * 32) + c8;
-    const int64_t row = step * 128 + rg;
-    const uint16_t* at = base + row * ld + col;
-    if (step * 128 + 128 <= p.M && col - c8 + 32 <= C) {
+    const int C = isg ? p.N : p.K, col = isg ? n0 + strip * 32 : k0 + (strip - TN / 32) * 32;
+    if (col >= C) return;                                 // (whole strips behind the last column: cut from what is there, never stored)
+    const uint16_t* base = (const uint16_t*)(isg ? p.g : p.x);
+    const int64_t left = p.M - (step + 1) * 128;          // rows behind this step
+    if (left >= 0 && (col + 32 <= C || left * ld >= 7)) {
+      // Columns stand alone, so what a lane reads behind the last one does not matter as long as it is memory of the tensor: pieces that
+      // begin behind it read the last piece instead, and the last piece's seven values too many lie in the rows behind (ld >= C).
+      const uint32_t off = 2 * ((uint32_t)rg * (uint32_t)ld + (uint32_t)min(c8, (C - 1 - col) & ~7));       // bytes; ld < 2^26
 #pragma unroll
-      for (int i = 0; i < 8; ++i) __builtin_memcpy(&v[i], at + i * 16 * ld, 16);
-    } else {
+      for (int i = 0; i < 8; ++i) __builtin_memcpy(&v[i], (const uint8_t*)(base + (step * 128 + i * 16) * ld + col) + off, 16);
+    } else {               // the tensor's end: every address held inside it, rows behind the last one zero (through LDS: few registers)
+      uint16_t* own = spare + tid * 8;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { Eight<T> e; e.load(at + i * 16 * ld, 0, row + i * 16 < p.M ? C - col : 0); v[i] = e.v; }
+      for (int i = 0; i < 8; ++i) {
+        const int64_t row = step * 128 + rg + i * 16;
+        const uint16_t* at = base + min(row, p.M - 1) * ld;
+#pragma clang loop unroll(disable)
+        for (int j = 0; j < 8; ++j) { const uint16_t e = at[min(col + c8 + j, C - 1)]; own[j] = row < p.M ? e : (uint16_t)0; }
+        v[i] = *(const u16x8*)own;
+      }
     }
   };
   auto cut = [&](int64_t step, int strip) __attribute__((always_inline)) {
@@ -639,49 +665,52 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
     const int buf = (int)(step - s0) & 1;
     uint8_t* t = smem8 + (buf * COLS + strip * 32) * 128;
     float* sc = scales + buf * COLS + strip * 32;
-    if (strip < TN / 32) tn_quant<T, FG>(v, t, sc, lane);
+    if (FG != F8_E4M3 && strip < TN / 32) tn_quant<T, FG>(v, t, sc, lane);
     else tn_quant<T, F8_E4M3>(v, t, sc, lane);
   };
+  // Waves 4 .. 7 sit on the same SIMDs as 0 .. 3: with a lower priority they fall behind, and one of a pair multiplies while the other cuts.
+  if (wave < 4) __builtin_amdgcn_s_setprio(1);
   load(s0, wave);
-  cut(s0, wave);
-  load(s0, wave + 8);
-  cut(s0, wave + 8);
-  load(s0 + 1, wave);
-  __syncthreads();
-  for (int64_t s = s0; s < s1; ++s) {
-    const int buf = (int)(s - s0) & 1;
-    const uint8_t* gt = smem8 + (buf * COLS + wn * 32 * NI + r) * 128;
-    const uint8_t* xt = smem8 + (buf * COLS + TN + wk * 64 + r) * 128;
-    const float* sc = scales + buf * COLS;
-    float sg[NI], sx[2];
+  const int64_t halves = 2 * (s1 - s0 + 1);
+  for (int64_t u = 0; u < halves; ++u) {     // two halves to a step: half of step s0 + u / 2 - 1 is multiplied, a strip of step s0 + u / 2 cut
+    const int half = (int)u & 1;
+    const int64_t next = s0 + (u >> 1);
+    if (u >= 2) {
+      const int buf = (int)(next - 1 - s0) & 1;
+      const uint8_t* gt = smem8 + (buf * COLS + wn * 32 * NI + r) * 128;
+      const uint8_t* xt = smem8 + (buf * COLS + TN + wk * 64 + r) * 128;
+      const float* sc = scales + buf * COLS;
+      float sg[NI], sx[2];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) sg[i] = sc[wn * 32 * NI + 32 * i + r];
+      for (int i = 0; i < NI; ++i) sg[i] = sc[wn * 32 * NI + 32 * i + r];
 #pragma unroll
-    for (int j = 0; j < 2; ++j) sx[j] = sc[TN + wk * 64 + 32 * j + r];
+      for (int j = 0; j < 2; ++j) sx[j] = sc[TN + wk * 64 + 32 * j + r];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int off = ((4 * h + c) ^ (r & 7)) * 16;
-      i32x4 fg[NI], fx[2];
+      for (int c = 0; c < 2; ++c) {
+        const int off = ((4 * h + 2 * half + c) ^ (r & 7)) * 16;
+        i32x4 fg[NI], fx[2];
 #pragma unroll
-      for (int i = 0; i < NI; ++i) fg[i] = *(const i32x4*)(gt + i * 4096 + off);
+        for (int i = 0; i < NI; ++i) fg[i] = *(const i32x4*)(gt + i * 4096 + off);
 #pragma unroll
-      for (int j = 0; j < 2; ++j) fx[j] = *(const i32x4*)(xt + j * 4096 + off);
+        for (int j = 0; j < 2; ++j) fx[j] = *(const i32x4*)(xt + j * 4096 + off);
 #pragma unroll
-      for (int q = 0; q < 2; ++q) {
-        b16x8 bx[2];
+        for (int q = 0; q < 2; ++q) {
+          b16x8 bx[2];
 #pragma unroll
-        for (int j = 0; j < 2; ++j) bx[j] = widen8<F8_E4M3>(fx[j][2 * q], fx[j][2 * q + 1], sx[j]);
+          for (int j = 0; j < 2; ++j) bx[j] = widen8<F8_E4M3>(fx[j][2 * q], fx[j][2 * q + 1], sx[j]);
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const b16x8 bg = widen8<FG>(fg[i][2 * q], fg[i][2 * q + 1], sg[i]);
+          for (int i = 0; i < NI; ++i) {
+            const b16x8 bg = widen8<FG>(fg[i][2 * q], fg[i][2 * q + 1], sg[i]);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bg, bx[j], acc[i][j], 0, 0, 0);
+            for (int j = 0; j < 2; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(bg, bx[j], acc[i][j], 0, 0, 0);
+          }
         }
+        __builtin_amdgcn_sched_barrier(0);     // (or every fragment of the half is read ahead, and registers spill)
       }
-      if (c == 1) { cut(s + 1, wave); load(s + 1, wave + 8); }
-      if (c == 3) { cut(s + 1, wave + 8); load(s + 2, wave); }
     }
-    __syncthreads();            // this step's tile has been read, the next one is written
+    cut(next, wave + 8 * half);
+    load(next + half, wave + 8 - 8 * half);
+    if (half) __syncthreads();            // the step has been read, the next one is written
   }
   float* y = p.y + (int64_t)part * p.N * p.K;
 #pragma unroll
@@ -873,7 +902,7 @@ extern "C" int64_t aln_fp8_grad_weight_ws_bytes(int64_t M, int32_t N, int32_t K,
   return up16(((int64_t)N + K) * per_row) + 16 * 4 + aln_fp8_nt_ws_bytes(N, K, M);
 }
 template <int T, int FG, int NI> static int tn_launch(const Fp8TN& p, int parts, hipStream_t st) {
-  constexpr int COLS = 64 * NI + 256, LDS = 2 * COLS * 132;
+  constexpr int COLS = 64 * NI + 256, LDS = 2 * COLS * 132 + 512 * 16;
   static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_grad_weight: %s", hipGetErrorString(big));
   const int64_t g = (int64_t)(parts + 7) / 8 * 8 * p.tn * p.tk;
@@ -889,8 +918,8 @@ template <int T> static int tn_pick(const Fp8TN& p, const TnPlan& t, int fmt_g, 
 extern "C" int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, int32_t fmt_g, const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t N, int32_t K,
                                    float* dw, void* ws, int64_t ws_bytes, void* stream) {
   ALN_REQUIRE(is_ft(g_type) && is_ft(x_type) && is_f8(fmt_g), "fp8_grad_weight: unknown type %d, %d or format %d", g_type, x_type, fmt_g);
-  ALN_REQUIRE(M >= 1 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldg >= 0 && ldx >= 0, "fp8_grad_weight: sizes %lld x %d x %d, pitches %lld, %lld", (long long)M, N, K,
-              (long long)ldg, (long long)ldx);
+  ALN_REQUIRE(M >= 1 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldg >= N && ldx >= K && ldg < 1 << 26 && ldx < 1 << 26,
+              "fp8_grad_weight: sizes %lld x %d x %d, pitches %lld, %lld (at least the columns, under 2^26)", (long long)M, N, K, (long long)ldg, (long long)ldx);
   ALN_REQUIRE(g && ((uintptr_t)g & (g_type == FT_F32 ? 3 : 1)) == 0 && x && ((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0 && dw && ((uintptr_t)dw & 3) == 0,
               "fp8_grad_weight: g, x or dw is NULL or not aligned to its type");
   const int64_t need = aln_fp8_grad_weight_ws_bytes(M, N, K, g_type, x_type);

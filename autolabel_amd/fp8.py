@@ -169,6 +169,8 @@ def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True)
     if need_dx:
         dx = linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt).reshape(x.shape)
     if need_dw:
+        # (rows that overlap, as an expanded gradient's do, or lie very far apart)
+        gr, xr = (t if t.shape[0] <= 1 or t.shape[1] <= t.stride(0) < 1 << 26 else t.contiguous() for t in (gr, xr))
         with _on(gr, xr):
             (m, n), k = gr.shape, xr.shape[1]
             if m == 0:
