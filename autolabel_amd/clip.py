@@ -32,38 +32,39 @@ def _dense(t):
 
 
 def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
-    grads = [grads] if torch.is_tensor(grads) else list(grads)
-    if not grads:
-        raise ValueError(f'{name}: an empty list of tensors')
-    dev = getattr(grads[0], 'device', None)
-    for i, t in enumerate(grads):
-        if not torch.is_tensor(t) or t.dtype not in TYPES or t.layout != torch.strided:
-            raise ValueError(f'{name}: tensor {i} must be a dense fp16, bf16 or fp32 tensor')
-        if not _dense(t):
-            raise ValueError(f'{name}: tensor {i} with shape {tuple(t.shape)} and strides {t.stride()} does not fill one run of memory')
-        if t.device != dev:
-            raise ValueError(f'{name}: tensors on different devices: {dev} and {t.device}')
-    if out is not None:
-        out = [out] if torch.is_tensor(out) else list(out)
-        if len(out) != len(grads):
-            raise ValueError(f'{name}: {len(grads)} tensors, {len(out)} outputs')
-        for i, (t, o) in enumerate(zip(grads, out)):
-            if o.dtype != t.dtype or o.shape != t.shape or o.device != dev or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous())):
-                raise ValueError(f'{name}: output {i} must have the type, shape, strides and device of its tensor')
-    for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32)):
-        if w is not None and (not torch.is_tensor(w) or w.dtype != dt or w.numel() < 1 or w.device != dev):
-            raise ValueError(f'{name}: {what} must be a device tensor of {dt} beside the gradients')
-    if not dev.type == 'cuda':
-        raise ValueError(f'{name}: autolabel_amd.clip has no CPU path: needs device tensors')
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
     n = len(grads)
-    with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
+    if not n:
+        raise ValueError(f'{name}: an empty list of tensors')
+    for i, t in enumerate(grads):
+        if not isinstance(t, torch.Tensor) or t.dtype not in TYPES or t.layout is not torch.strided:
+            raise ValueError(f'{name}: tensor {i} must be a dense fp16, bf16 or fp32 tensor')
+        if not t.is_contiguous() and not _dense(t):
+            raise ValueError(f'{name}: tensor {i} with shape {tuple(t.shape)} and strides {t.stride()} does not fill one run of memory')
+    index = [t.get_device() for t in grads]
+    dev = grads[0].device
+    if index.count(index[0]) != n:
+        raise ValueError(f'{name}: tensors on different devices: {", ".join(sorted({str(t.device) for t in grads}))}')
+    to = None
+    if out is not None:
+        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        if len(out) != n:
+            raise ValueError(f'{name}: {n} tensors, {len(out)} outputs')
+        for i, (t, o) in enumerate(zip(grads, out)):
+            if o.dtype is not t.dtype or o.shape != t.shape or o.get_device() != index[0] or (not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride()):
+                raise ValueError(f'{name}: output {i} must have the type, shape, strides and device of its tensor')
+        to = (C.c_void_p * n)(*[o.data_ptr() for o in out])
+    for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32)):
+        if w is not None and (not isinstance(w, torch.Tensor) or w.dtype != dt or w.numel() < 1 or w.device != dev):
+            raise ValueError(f'{name}: {what} must be a device tensor of {dt} beside the gradients')
+    if index[0] < 0:
+        raise ValueError(f'{name}: autolabel_amd.clip has no CPU path: needs device tensors')
+    with contextlib.nullcontext() if index[0] == torch.cuda.current_device() else torch.cuda.device(dev):
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = torch.empty(int(H.lib().aln_grad_clip_ws_bytes(n)), dtype=torch.uint8, device=dev)
-        pointers = C.c_void_p * n
-        H.call('aln_grad_clip', n, pointers(*[t.data_ptr() for t in grads]), pointers(*[t.data_ptr() for t in out]) if out is not None else None,
-               (C.c_int64 * n)(*[t.numel() for t in grads]), (C.c_int32 * n)(*[TYPES[t.dtype] for t in grads]), max_norm, int(apply),
-               H.C.c_void_p(loss_scale.data_ptr()) if loss_scale is not None else None, H.C.c_void_p(norm.data_ptr()),
-               H.C.c_void_p(found_inf.data_ptr()) if found_inf is not None else None, H.C.c_void_p(ws.data_ptr()), ws.numel(), H.stream())
+        ws = torch.empty(H.lib().aln_grad_clip_ws_bytes(n), dtype=torch.uint8, device=dev)
+        H.call('aln_grad_clip', n, (C.c_void_p * n)(*[t.data_ptr() for t in grads]), to, (C.c_int64 * n)(*[t.numel() for t in grads]),
+               (C.c_int32 * n)(*[TYPES[t.dtype] for t in grads]), max_norm, int(apply), loss_scale.data_ptr() if loss_scale is not None else None,
+               norm.data_ptr(), found_inf.data_ptr() if found_inf is not None else None, ws.data_ptr(), ws.numel(), H.raw_stream())
     return norm
 
 

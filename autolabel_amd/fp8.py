@@ -53,7 +53,7 @@ class Fp8Blocks:
         q, s = self.q, self.scale
         if self.cols < 1 or q.dim() != 2 or q.dtype != FORMATS[self.fmt][1] or not q.is_contiguous() or q.shape[1] < nb * BLOCK or q.shape[1] % 16:
             raise ValueError(f'{name}: q must be contiguous {FORMATS[self.fmt][1]} [rows, whole blocks of 128 for {self.cols} columns], got {q.dtype} {tuple(q.shape)}')
-        if s.dim() != 2 or s.dtype != torch.uint8 or not s.is_contiguous() or s.shape[0] != q.shape[0] or s.shape[1] < nb or s.shape[1] % 4 or s.device != q.device:
+        if s.dim() != 2 or s.dtype != torch.uint8 or not s.is_contiguous() or s.shape[0] != q.shape[0] or s.shape[1] < nb or s.shape[1] % 4 or s.get_device() != q.get_device():
             raise ValueError(f'{name}: scale must be contiguous uint8 [rows, a multiple of 4 >= {nb}] beside q, got {s.dtype} {tuple(s.shape)}')
 
 
@@ -64,13 +64,15 @@ def _need(ok, message):
 
 def _rows(name, x):
     """x as [rows, columns] with unit column stride (a view where its strides allow one, else a copy)."""
-    _need(torch.is_tensor(x) and x.dtype in TYPES, f'{name}: needs an fp16, bf16 or fp32 tensor')
-    _need(x.dim() >= 1 and x.shape[-1] >= 1, f'{name}: needs at least one column, got shape {tuple(x.shape)}')
-    x = x.detach()
-    if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
-    if x.shape[1] > 1 and x.stride(1) != 1:
-        x = x.contiguous()
+    if not isinstance(x, torch.Tensor) or x.dtype not in TYPES:
+        raise ValueError(f'{name}: needs an fp16, bf16 or fp32 tensor')
+    shape = x.shape
+    if not shape or not shape[-1]:
+        raise ValueError(f'{name}: needs at least one column, got shape {tuple(shape)}')
+    if len(shape) != 2:
+        x = x.detach().reshape(-1, shape[-1])
+    if x.stride(1) != 1 and shape[-1] > 1:
+        x = x.detach().contiguous()
     return x
 
 
@@ -78,13 +80,17 @@ def _pitch(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
-def _on(*tensors):
+_NOTHING = contextlib.nullcontext()
+
+
+def _on(a, b=None):
     """The tensors' common device made current (a no-op where it is)."""
-    dev = tensors[0].device
-    for t in tensors:
-        _need(t.is_cuda, 'autolabel_amd.fp8 has no CPU path: needs device tensors')
-        _need(t.device == dev, f'tensors on different devices: {dev} and {t.device}')
-    return contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+    i = a.get_device()
+    if i < 0 or (b is not None and b.get_device() != i):
+        if i < 0 or b.get_device() < 0:
+            raise ValueError('autolabel_amd.fp8 has no CPU path: needs device tensors')
+        raise ValueError(f'tensors on different devices: {a.device} and {b.device}')
+    return _NOTHING if i == torch.cuda.current_device() else torch.cuda.device(i)
 
 
 def _p(t):
@@ -107,7 +113,7 @@ def quantize(x, fmt='e4m3', transpose=False):
     with _on(x):
         out = _empty_blocks(k, m, fmt, x.device) if transpose else _empty_blocks(m, k, fmt, x.device)
         H.call('aln_fp8_quantize_t' if transpose else 'aln_fp8_quantize', _p(x), TYPES[x.dtype], _pitch(x), m, k, FORMATS[fmt][0], _p(out.q),
-               out.q.shape[1], _p(out.scale), out.scale.shape[1], H.stream())
+               out.q.shape[1], _p(out.scale), out.scale.shape[1], H.raw_stream())
     return out
 
 
@@ -128,7 +134,7 @@ def matmul(a, b, out_dtype=torch.float16, relu=False):
         nbytes = int(H.lib().aln_fp8_nt_ws_bytes(m, n, k))
         ws = torch.empty(nbytes, dtype=torch.uint8, device=a.q.device) if nbytes else None
         H.call('aln_fp8_nt', _p(a.q), a.q.shape[1], _p(a.scale), a.scale.shape[1], FORMATS[a.fmt][0], _p(b.q), b.q.shape[1], _p(b.scale),
-               b.scale.shape[1], FORMATS[b.fmt][0], m, n, k, _p(y), n, TYPES[out_dtype], int(bool(relu)), _p(ws) if nbytes else None, nbytes, H.stream())
+               b.scale.shape[1], FORMATS[b.fmt][0], m, n, k, _p(y), n, TYPES[out_dtype], int(bool(relu)), _p(ws) if nbytes else None, nbytes, H.raw_stream())
     return y
 
 
@@ -149,7 +155,7 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         H.call('aln_fp8_linear', _p(rows), TYPES[x.dtype], _pitch(rows), FORMATS[fmt][0], _p(weight.q), weight.q.shape[1], _p(weight.scale),
                weight.scale.shape[1], FORMATS[weight.fmt][0], m, n, k, _p(y), n, TYPES[out_dtype], int(bool(relu)), _p(ws) if nbytes else None, nbytes,
-               H.stream())
+               H.raw_stream())
     return y
 
 
@@ -179,7 +185,7 @@ def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True)
             nbytes = H.lib().aln_fp8_grad_weight_ws_bytes(m, n, k, TYPES[g.dtype], TYPES[x.dtype])
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
             H.call('aln_fp8_grad_weight', _p(gr), TYPES[g.dtype], _pitch(gr), FORMATS[grad_fmt][0], _p(xr), TYPES[x.dtype], _pitch(xr), m, n, k,
-                   _p(dw), _p(ws) if nbytes else None, nbytes, H.stream())
+                   _p(dw), _p(ws) if nbytes else None, nbytes, H.raw_stream())
     return dx, dw
 
 
