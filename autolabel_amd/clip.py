@@ -7,9 +7,10 @@ pass and the optimizer: ``TrainEngine(max_grad_norm=...)`` / ``Trainer(max_grad_
 
 One launch for the squares and one for the scaling per 120 tensors, whatever their sizes and types; the norm stays on the device.
 """
+import array
 import contextlib
-import ctypes as C
 import math
+import operator
 
 import torch
 
@@ -31,40 +32,58 @@ def _dense(t):
     return True
 
 
+# Unbound methods mapped over the lists: a list of 60 small gradients costs more on the host than on the device.
+_T = torch.Tensor
+_dtype = operator.attrgetter('dtype')
+
+
+def _check(name, grads, out, loss_scale, found_inf):
+    """Say what is wrong with the arguments (the slow way: one is known to be)."""
+    dev = getattr(grads[0], 'device', None)
+    for i, t in enumerate(grads):
+        if not torch.is_tensor(t) or t.layout != torch.strided or t.dtype not in TYPES:
+            raise ValueError(f'{name}: tensor {i} must be a dense fp16, bf16 or fp32 tensor')
+        if not _dense(t):
+            raise ValueError(f'{name}: tensor {i} with shape {tuple(t.shape)} and strides {t.stride()} does not fill one run of memory')
+        if t.device != dev:
+            raise ValueError(f'{name}: tensors on different devices: {dev} and {t.device}')
+    for i, (t, o) in enumerate(zip(grads, out or ())):
+        if not torch.is_tensor(o) or o.dtype != t.dtype or o.shape != t.shape or o.device != dev or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous())):
+            raise ValueError(f'{name}: output {i} must have the type, shape, strides and device of its tensor')
+    for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32)):
+        if w is not None and (not torch.is_tensor(w) or w.dtype != dt or w.numel() < 1 or w.device != dev):
+            raise ValueError(f'{name}: {what} must be a device tensor of {dt} beside the gradients')
+    if dev.type != 'cuda':
+        raise ValueError(f'{name}: autolabel_amd.clip has no CPU path: needs device tensors')
+
+
 def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
-    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    grads = [grads] if torch.is_tensor(grads) else list(grads)
     n = len(grads)
     if not n:
         raise ValueError(f'{name}: an empty list of tensors')
-    for i, t in enumerate(grads):
-        if not isinstance(t, torch.Tensor) or t.dtype not in TYPES or t.layout is not torch.strided:
-            raise ValueError(f'{name}: tensor {i} must be a dense fp16, bf16 or fp32 tensor')
-        if not t.is_contiguous() and not _dense(t):
-            raise ValueError(f'{name}: tensor {i} with shape {tuple(t.shape)} and strides {t.stride()} does not fill one run of memory')
-    index = [t.get_device() for t in grads]
-    dev = grads[0].device
-    if index.count(index[0]) != n:
-        raise ValueError(f'{name}: tensors on different devices: {", ".join(sorted({str(t.device) for t in grads}))}')
-    to = None
     if out is not None:
-        out = [out] if isinstance(out, torch.Tensor) else list(out)
+        out = [out] if torch.is_tensor(out) else list(out)
         if len(out) != n:
             raise ValueError(f'{name}: {n} tensors, {len(out)} outputs')
-        for i, (t, o) in enumerate(zip(grads, out)):
-            if o.dtype is not t.dtype or o.shape != t.shape or o.get_device() != index[0] or (not (o.is_contiguous() and t.is_contiguous()) and o.stride() != t.stride()):
-                raise ValueError(f'{name}: output {i} must have the type, shape, strides and device of its tensor')
-        to = (C.c_void_p * n)(*[o.data_ptr() for o in out])
-    for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32)):
-        if w is not None and (not isinstance(w, torch.Tensor) or w.dtype != dt or w.numel() < 1 or w.device != dev):
-            raise ValueError(f'{name}: {what} must be a device tensor of {dt} beside the gradients')
-    if index[0] < 0:
-        raise ValueError(f'{name}: autolabel_amd.clip has no CPU path: needs device tensors')
-    with contextlib.nullcontext() if index[0] == torch.cuda.current_device() else torch.cuda.device(dev):
+    every = grads if out is None else grads + out
+    good = all(map(torch.is_tensor, every)) and all(map(_T.is_contiguous, every))
+    if good:
+        types, device = list(map(_dtype, grads)), list(map(_T.get_device, every))
+        good = device[0] >= 0 and device.count(device[0]) == len(every) and TYPES.keys() >= set(types)
+        good = good and (out is None or (list(map(_dtype, out)) == types and list(map(_T.size, out)) == list(map(_T.size, grads))))
+    if not good or loss_scale is not None or found_inf is not None:
+        _check(name, grads, out, loss_scale, found_inf)
+        types = list(map(_dtype, grads))
+    dev = grads[0].device
+    with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
         norm = torch.empty((), dtype=torch.float32, device=dev)
         ws = torch.empty(H.lib().aln_grad_clip_ws_bytes(n), dtype=torch.uint8, device=dev)
-        H.call('aln_grad_clip', n, (C.c_void_p * n)(*[t.data_ptr() for t in grads]), to, (C.c_int64 * n)(*[t.numel() for t in grads]),
-               (C.c_int32 * n)(*[TYPES[t.dtype] for t in grads]), max_norm, int(apply), loss_scale.data_ptr() if loss_scale is not None else None,
-               norm.data_ptr(), found_inf.data_ptr() if found_inf is not None else None, ws.data_ptr(), ws.numel(), H.raw_stream())
+        g, o = array.array('Q', map(_T.data_ptr, grads)), None if out is None else array.array('Q', map(_T.data_ptr, out))
+        sizes, types = array.array('q', map(_T.numel, grads)), array.array('i', map(TYPES.__getitem__, types))
+        H.call('aln_grad_clip', n, g.buffer_info()[0], None if o is None else o.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], max_norm,
+               int(apply), loss_scale.data_ptr() if loss_scale is not None else None, norm.data_ptr(),
+               found_inf.data_ptr() if found_inf is not None else None, ws.data_ptr(), ws.numel(), H.raw_stream())
     return norm
 
 

@@ -322,74 +322,79 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
     for (int j = 0; j < MI; ++j)
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  constexpr int PIECES = ROWS / 8 / NW;                   // direct copies of a wave per step, eight rows each
   const int sub = lane >> 3, slot = lane & 7;
-  auto fetch = [&](int kb, int buf) {
+  const uint8_t* src[PIECES];
 #pragma unroll
-    for (int i = 0; i < ROWS / 8 / NW; ++i) {
-      const int row = (wave + i * NW) * 8 + sub;       // row of the tile: A's first, then B's (a wave's eight rows are all of one kind)
-      const uint8_t* src = row < BM ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (int64_t)min(n0 + row - BM, p.N - 1) * p.ldb;
-      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src + (int64_t)kb * 128 + ((slot ^ (row & 7)) * 16)),
+  for (int i = 0; i < PIECES; ++i) {
+    const int row = (wave + i * NW) * 8 + sub;            // row of the tile: A's first, then B's (a wave's eight rows are all of one kind)
+    src[i] = (row < BM ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (int64_t)min(n0 + row - BM, p.N - 1) * p.ldb) + (int64_t)kb0 * 128 + ((slot ^ (row & 7)) * 16);
+  }
+  auto fetch = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src[i],
                                        (__attribute__((address_space(3))) void*)(smem8 + buf * ROWS * 128 + (wave + i * NW) * 1024), 16, 0, 0);
+      src[i] += 128;
     }
   };
+  // scales: a word holds four blocks of a row; the next word is sent for when the current one is begun (parts begin at multiples of four)
   const uint8_t *pa[MI], *pb[NI];
+  uint32_t sa[MI], sb[NI], na[MI], nb[NI];
 #pragma unroll
-  for (int j = 0; j < MI; ++j) pa[j] = p.sa + min(m0 + (wm * MI + j) * 32 + r, p.M - 1) * p.ldsa;
+  for (int j = 0; j < MI; ++j) { pa[j] = p.sa + min(m0 + (wm * MI + j) * 32 + r, p.M - 1) * p.ldsa + kb0; na[j] = *(const uint32_t*)pa[j]; }
 #pragma unroll
-  for (int i = 0; i < NI; ++i) pb[i] = p.sb + (int64_t)min(n0 + (wn * NI + i) * 32 + r, p.N - 1) * p.ldsb;
-  int sa[MI], sb[NI];
-  auto scales = [&](int kb) {
+  for (int i = 0; i < NI; ++i) { pb[i] = p.sb + (int64_t)min(n0 + (wn * NI + i) * 32 + r, p.N - 1) * p.ldsb + kb0; nb[i] = *(const uint32_t*)pb[i]; }
+  int off[4];
 #pragma unroll
-    for (int j = 0; j < MI; ++j) sa[j] = pa[j][kb];
+  for (int c = 0; c < 4; ++c) off[c] = r * 128 + (((4 * h + c) ^ (r & 7)) * 16);
+  fetch(0);
+  __syncthreads();
+  for (int kb = kb0; kb < kb1; ++kb) {
+    const int buf = (kb - kb0) & 1;
+    if (((kb - kb0) & 3) == 0) {
+      const bool more = kb + 4 < kb1;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) sb[i] = pb[i][kb];
-  };
-  if (kb0 < kb1) {
-    fetch(kb0, 0);
-    __syncthreads();
-    for (int kb = kb0; kb < kb1; ++kb) {
-      const int buf = (kb - kb0) & 1;
-      scales(kb);
-      if (kb + 1 < kb1) fetch(kb + 1, buf ^ 1);
-      const uint8_t* t = smem8 + buf * ROWS * 128;
+      for (int j = 0; j < MI; ++j) { sa[j] = na[j]; if (more) { pa[j] += 4; na[j] = *(const uint32_t*)pa[j]; } }
 #pragma unroll
-      for (int ks = 0; ks < 2; ++ks) {
-        i32x8 fa[MI], fb[NI];
-        const int c0 = 4 * h + 2 * ks;
-#pragma unroll
-        for (int j = 0; j < MI; ++j) {
-          const uint8_t* row = t + ((wm * MI + j) * 32 + r) * 128;
-          const i32x4 lo = *(const i32x4*)(row + ((c0 ^ (r & 7)) * 16)), hi = *(const i32x4*)(row + (((c0 + 1) ^ (r & 7)) * 16));
-          fa[j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-#pragma unroll
-        for (int i = 0; i < NI; ++i) {
-          const uint8_t* row = t + (BM + (wn * NI + i) * 32 + r) * 128;
-          const i32x4 lo = *(const i32x4*)(row + ((c0 ^ (r & 7)) * 16)), hi = *(const i32x4*)(row + (((c0 + 1) ^ (r & 7)) * 16));
-          fb[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        }
-        if constexpr (WIDE) {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            b16x8 xa[MI];
-#pragma unroll
-            for (int j = 0; j < MI; ++j) xa[j] = widen8<FA>(fa[j][2 * q], fa[j][2 * q + 1], __uint_as_float((uint32_t)sa[j] << 23));
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-              const b16x8 xb = widen8<FB>(fb[i][2 * q], fb[i][2 * q + 1], __uint_as_float((uint32_t)sb[i] << 23));
-#pragma unroll
-              for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb, xa[j], acc[i][j], 0, 0, 0);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int j = 0; j < MI; ++j) acc[i][j] = mfma8<FB, FA>(fb[i], fa[j], acc[i][j], sb[i], sa[j]);
-        }
-      }
-      __syncthreads();          // the tile has been read, the next one has landed
+      for (int i = 0; i < NI; ++i) { sb[i] = nb[i]; if (more) { pb[i] += 4; nb[i] = *(const uint32_t*)pb[i]; } }
     }
+    if (kb + 1 < kb1) fetch(buf ^ 1);
+    const uint8_t *ta = smem8 + buf * ROWS * 128 + wm * MI * 4096, *tb = smem8 + buf * ROWS * 128 + BM * 128 + wn * NI * 4096;
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      i32x8 fa[MI], fb[NI];
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        fb[i] = __builtin_shufflevector(*(const i32x4*)(tb + i * 4096 + off[2 * ks]), *(const i32x4*)(tb + i * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+      for (int j = 0; j < MI; ++j)
+        fa[j] = __builtin_shufflevector(*(const i32x4*)(ta + j * 4096 + off[2 * ks]), *(const i32x4*)(ta + j * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+      if constexpr (WIDE) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          b16x8 xa[MI];
+#pragma unroll
+          for (int j = 0; j < MI; ++j) xa[j] = widen8<FA>(fa[j][2 * q], fa[j][2 * q + 1], __uint_as_float((sa[j] & 255u) << 23));
+#pragma unroll
+          for (int i = 0; i < NI; ++i) {
+            const b16x8 xb = widen8<FB>(fb[i][2 * q], fb[i][2 * q + 1], __uint_as_float((sb[i] & 255u) << 23));
+#pragma unroll
+            for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb, xa[j], acc[i][j], 0, 0, 0);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < MI; ++j)
+#pragma unroll
+          for (int i = 0; i < NI; ++i) acc[i][j] = mfma8<FB, FA>(fb[i], fa[j], acc[i][j], (int)sb[i], (int)sa[j]);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < MI; ++j) sa[j] >>= 8;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sb[i] >>= 8;
+    __syncthreads();            // the tile has been read, the next one has landed
   }
   Fp8Out o = p.o;
   if (p.splits > 1) { o.y = (float*)o.y + (int64_t)blockIdx.y * p.M * p.N; o.ldy = p.N; o.type = FT_F32; o.relu = 0; }
@@ -808,7 +813,7 @@ static NtPlan nt_plan(int64_t M, int N, int64_t K) {
   int64_t s = tiles >= 256 ? 1 : 512 / tiles;
   if (s > nkb / 4) s = nkb / 4;
   if (s < 1) s = 1;
-  const int64_t per = (nkb + s - 1) / s;
+  const int64_t per = ((nkb + s - 1) / s + 3) / 4 * 4;    // (whole words of scales)
   return {(int)((nkb + per - 1) / per), (int)per};
 }
 extern "C" int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K) {
@@ -816,16 +821,20 @@ extern "C" int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K) {
   const NtPlan pl = nt_plan(M, N, K);
   return pl.splits > 1 ? (int64_t)pl.splits * M * N * 4 : 0;
 }
-template <int FA, int FB, bool WIDE> static int nt_launch(Fp8NT& p, hipStream_t st) {
-  constexpr int WM = 2, WN = 2, MI = 2, NI = 2, BM = WM * MI * 32, BN = WN * NI * 32;
+template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI> static int nt_launch(const Fp8NT& p, hipStream_t st) {
+  constexpr int BM = WM * MI * 32, BN = WN * NI * 32, LDS = 2 * (BM + BN) * 128;
+  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  ALN_REQUIRE(big == hipSuccess, "fp8_nt: %s", hipGetErrorString(big));
   const int64_t g = ((p.M + BM - 1) / BM + 7) / 8 * 8 * ((p.N + BN - 1) / BN);
   ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_nt: %lld x %d results are too many for one launch", (long long)p.M, p.N);
-  hipLaunchKernelGGL((k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>), dim3((uint32_t)g, p.splits), dim3(64 * WM * WN), 2 * (BM + BN) * 128, st, p);
+  hipLaunchKernelGGL((k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>), dim3((uint32_t)g, p.splits), dim3(64 * WM * WN), LDS, st, p);
   ALN_CHECK_LAUNCH("fp8_nt");
   return 0;
 }
-template <int FA, int FB> static int nt_type(Fp8NT& p, int y_type, hipStream_t st) {
-  return y_type == FT_F32 ? nt_launch<FA, FB, true>(p, st) : nt_launch<FA, FB, false>(p, st);
+template <int FA, int FB> static int nt_type(const Fp8NT& p, int y_type, hipStream_t st) {
+  const bool big = (p.M + 255) / 256 * ((p.N + 255) / 256) >= 256;
+  if (y_type == FT_F32) return big ? nt_launch<FA, FB, true, 2, 4, 4, 2>(p, st) : nt_launch<FA, FB, true, 2, 2, 2, 2>(p, st);
+  return big ? nt_launch<FA, FB, false, 2, 4, 4, 2>(p, st) : nt_launch<FA, FB, false, 2, 2, 2, 2>(p, st);
 }
 extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t ldsa, int32_t fmt_a, const void* b, int64_t ldb, const uint8_t* sb, int64_t ldsb,
                           int32_t fmt_b, int64_t M, int32_t N, int64_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws, int64_t ws_bytes,
