@@ -291,6 +291,9 @@ __device__ inline void store_block(const Fp8Out& o, const f32x16& c0, const f32x
   __builtin_amdgcn_wave_barrier();
 }
 
+// The slot of piece c of row r in a tile of 128-byte rows is c ^ turn(r)
+__device__ inline int turn(int row) { return (row >> 1) & 7; }
+
 struct Fp8NT {
   const uint8_t* a; int64_t lda; const uint8_t* sa; int64_t ldsa;   // [M, K] rows of y
   const uint8_t* b; int64_t ldb; const uint8_t* sb; int64_t ldsb;   // [N, K] columns of y
@@ -328,7 +331,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
 #pragma unroll
   for (int i = 0; i < PIECES; ++i) {
     const int row = (wave + i * NW) * 8 + sub;            // row of the tile: A's first, then B's (a wave's eight rows are all of one kind)
-    src[i] = (row < BM ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (int64_t)min(n0 + row - BM, p.N - 1) * p.ldb) + (int64_t)kb0 * 128 + ((slot ^ (row & 7)) * 16);
+    src[i] = (row < BM ? p.a + min(m0 + row, p.M - 1) * p.lda : p.b + (int64_t)min(n0 + row - BM, p.N - 1) * p.ldb) + (int64_t)kb0 * 128 + ((slot ^ turn(row)) * 16);
   }
   auto fetch = [&](int buf) __attribute__((always_inline)) {
 #pragma unroll
@@ -347,7 +350,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
   for (int i = 0; i < NI; ++i) { pb[i] = p.sb + (int64_t)min(n0 + (wn * NI + i) * 32 + r, p.N - 1) * p.ldsb + kb0; nb[i] = *(const uint32_t*)pb[i]; }
   int off[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) off[c] = r * 128 + (((4 * h + c) ^ (r & 7)) * 16);
+  for (int c = 0; c < 4; ++c) off[c] = r * 128 + (((4 * h + c) ^ turn(r)) * 16);
   fetch(0);
   __syncthreads();
   for (int kb = kb0; kb < kb1; ++kb) {
@@ -451,7 +454,7 @@ __global__ __launch_bounds__(256, 2) void k_fp8_linear(Fp8Linear p) {
     for (int i = 0; i < 4; ++i) { w4[i] = *(const i32x4*)fp[i]; fp[i] += 128; }
     if (++fkb == nkb) { fkb = 0; ++ft; aim(); }
   };
-  const int put = wrow * 128 + ((piece ^ (wrow & 7)) * 16);
+  const int put = wrow * 128 + ((piece ^ turn(wrow)) * 16);
   auto stash = [&](int half, const i32x4 (&w4)[4]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) *(i32x4*)(ws + half * 16384 + put + i * 4096) = w4[i];
@@ -482,7 +485,7 @@ __global__ __launch_bounds__(256, 2) void k_fp8_linear(Fp8Linear p) {
           const BlockScale bs = block_scale<FX>(dpp_umax<0x4E>(dpp_umax<0xB1>(m)));
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            *(uint2*)(dst + (b0 + b) * 128 + (((2 * j + (l >> 1)) ^ (row & 7)) * 16) + (l & 1) * 8) = quant8<T, FX>(v[b][j], bs);
+            *(uint2*)(dst + (b0 + b) * 128 + (((2 * j + (l >> 1)) ^ turn(row)) * 16) + (l & 1) * 8) = quant8<T, FX>(v[b][j], bs);
           if (l == 0) se[row * LIN_NKB + b0 + b] = bs.byte;
         }
     }
@@ -504,7 +507,7 @@ __global__ __launch_bounds__(256, 2) void k_fp8_linear(Fp8Linear p) {
   const uint8_t* wr0 = ws + (wn * 64 + r) * 128;
   int off[4];
 #pragma unroll
-  for (int c = 0; c < 4; ++c) off[c] = ((4 * h + c) ^ (r & 7)) * 16;
+  for (int c = 0; c < 4; ++c) off[c] = ((4 * h + c) ^ turn(r)) * 16;
   int t = t0, kb = 0;
   auto one = [&](int half, i32x4 (&next)[4]) __attribute__((always_inline)) {            // `next` holds the tile of the next step
     if (kb == 0) {
@@ -609,7 +612,7 @@ template <int T, int FMT> __device__ inline void tn_quant(u16x8 (&v)[8], uint8_t
 #pragma unroll
     for (int i = 0; i < 4; ++i)        // column j of two rows in one word
       w[i] = __builtin_amdgcn_perm(__builtin_bit_cast(i32x4, v[2 * i + 1])[j / 2], __builtin_bit_cast(i32x4, v[2 * i])[j / 2], (j & 1) ? 0x07060302u : 0x05040100u);
-    *(uint2*)(tile + (c8 + j) * 128 + ((((rg >> 1) ^ j) * 16) | ((rg & 1) * 8))) = make_uint2(cvt4<T, FMT>(w[0], w[1], s[j]), cvt4<T, FMT>(w[2], w[3], s[j]));
+    *(uint2*)(tile + (c8 + j) * 128 + ((((rg >> 1) ^ turn(c8 + j)) * 16) | ((rg & 1) * 8))) = make_uint2(cvt4<T, FMT>(w[0], w[1], s[j]), cvt4<T, FMT>(w[2], w[3], s[j]));
   }
   if (rg == 0) { *(f32x4*)(scale + c8) = (f32x4){s[0], s[1], s[2], s[3]}; *(f32x4*)(scale + c8 + 4) = (f32x4){s[4], s[5], s[6], s[7]}; }
 }
@@ -693,7 +696,7 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
       for (int j = 0; j < 2; ++j) sx[j] = sc[TN + wk * 64 + 32 * j + r];
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int off = ((4 * h + 2 * half + c) ^ (r & 7)) * 16;
+        const int off = ((4 * h + 2 * half + c) ^ turn(r)) * 16;
         i32x4 fg[NI], fx[2];
 #pragma unroll
         for (int i = 0; i < NI; ++i) fg[i] = *(const i32x4*)(gt + i * 4096 + off);
