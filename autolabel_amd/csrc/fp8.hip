@@ -411,144 +411,146 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
     }
 }
 
-// y = x W^T with the rows of x cut into blocks on the way: 64 rows of x, all of their (up to 1024) columns, become 8-bit values in LDS once,
-// then the weights stream past them from L2 in tiles of 128 rows x 128 columns -- the values of x never exist in 8 bits in memory.
+// y = x W^T with the rows of x cut into blocks on the way; the values of x never exist in 8 bits in memory, and the weights never in LDS: a wave
+// keeps the 32 rows of W that it multiplies by -- all of their up to 1024 columns -- in registers (16 NKB of them) and lets x stream past.
+// Sixteen waves hold 512 x 512 weights (half of a CU's registers); above 512 columns eight waves hold 256 x 1024.  A block of threads owns a
+// range of rows and goes through it in tiles of up to 64: a tile's rows are cut into 8-bit blocks in one LDS buffer (four lanes to a block, its
+// power of two worked out once for 32 values) while the tile before it is multiplied out of the other and the loads of the one after it are in
+// flight.  One barrier per tile.
 struct Fp8Linear {
   const void* x; int64_t ldx;
   const uint8_t* w; int64_t ldw; const uint8_t* sw; int64_t ldsw;
-  int64_t M; int N, K, nkb;
-  int parts, per;                 // the columns of y in `parts` parts of `per` tiles of 128
+  int64_t M; int N, K;
+  int wn, parts;                  // waves side by side along the columns of y (a power of two); blocks of threads side by side
+  int rows, bm;                   // rows of a block of threads, of a tile (<= 64)
   Fp8Out o;
 };
-#define LIN_BM 64
 #define LIN_NKB 8
-static inline int lin_lds(int nkb) { return LIN_BM * nkb * 128 + 2 * 128 * 128 + LIN_BM * LIN_NKB; }
+template <int NKB> constexpr int lin_threads() { return NKB <= 4 ? 1024 : 512; }
 
-template <int T, int FX>
-__global__ __launch_bounds__(256, 2) void k_fp8_linear(Fp8Linear p) {
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];
-  uint8_t* xs = smem8;                                    // [64][nkb][128], pieces of 16 bytes turned by the row within each block
-  uint8_t* ws = xs + LIN_BM * p.nkb * 128;                // [2][128][128]
-  uint8_t* se = ws + 2 * 128 * 128;                       // [64][8] exponents + 127
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
-  const int wm = wave & 1, wn = wave >> 1, nkb = p.nkb;
-  // blocks b and b + 8 run on the same XCD: the parts of a row tile go there and share its rows in that L2
-  const int xcd = blockIdx.x & 7, jj = blockIdx.x >> 3;
-  const int64_t m0 = ((int64_t)(jj / p.parts) * 8 + xcd) * LIN_BM;
-  if (m0 >= p.M) return;
-  const int t0 = (jj % p.parts) * p.per, t1 = min((p.N + 127) / 128, t0 + p.per);
-  const int steps = (t1 - t0) * nkb;                      // >= 1
-  // The weights' tiles come through registers, two steps ahead of the one that is multiplied: a step's arithmetic is shorter than the way to
-  // L2.  The cursor (ft, fkb) runs over them; rows behind the last are clamped (their results are never stored).
-  i32x4 wa[4], wb[4];
-  const int wrow = tid >> 3, piece = tid & 7;             // rows wrow + 32 i of the tile, one 16-byte piece
-  const uint8_t* fp[4];
-  int ft = t0, fkb = 0;
-  auto aim = [&]() __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fp[i] = p.w + (int64_t)min(ft * 128 + wrow + 32 * i, p.N - 1) * p.ldw + piece * 16;
-  };
-  auto fetch = [&](i32x4 (&w4)[4]) __attribute__((always_inline)) {
-    if (ft >= t1) return;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { w4[i] = *(const i32x4*)fp[i]; fp[i] += 128; }
-    if (++fkb == nkb) { fkb = 0; ++ft; aim(); }
-  };
-  const int put = wrow * 128 + ((piece ^ turn(wrow)) * 16);
-  auto stash = [&](int half, const i32x4 (&w4)[4]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) *(i32x4*)(ws + half * 16384 + put + i * 4096) = w4[i];
-  };
-  aim();
-  fetch(wa);
-  fetch(wb);
-  // four lanes hold a block of a row, pieces l, l + 4, ... of eight values each: its maximum takes two exchanges, its power of two is worked
-  // out once for 32 values of a lane
-  {
-    const int row = tid >> 2, l = tid & 3;
-    const int64_t at = min(m0 + row, p.M - 1) * p.ldx;
-    uint8_t* dst = xs + row * nkb * 128;
-    for (int b0 = 0; b0 < nkb; b0 += 4) {
-      Eight<T> v[4][4];
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (b0 + b < nkb) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) { const int k = (b0 + b) * 128 + (4 * j + l) * 8; v[b][j].load(p.x, at + k, p.K - k); }
-        }
-#pragma unroll
-      for (int b = 0; b < 4; ++b)
-        if (b0 + b < nkb) {
-          uint32_t m = 0;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) { const uint32_t a = v[b][j].amax(); m = a > m ? a : m; }
-          const BlockScale bs = block_scale<FX>(dpp_umax<0x4E>(dpp_umax<0xB1>(m)));
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-            *(uint2*)(dst + (b0 + b) * 128 + (((2 * j + (l >> 1)) ^ turn(row)) * 16) + (l & 1) * 8) = quant8<T, FX>(v[b][j], bs);
-          if (l == 0) se[row * LIN_NKB + b0 + b] = bs.byte;
-        }
-    }
-  }
-  stash(0, wa);
-  fetch(wa);
-  // the weights' exponents, four blocks to a word, a group of four blocks ahead
-  const uint8_t* sp[2];
-  uint32_t sw_now[2] = {0, 0}, sw_next[2];
-  auto aim_scales = [&](int t) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) { sp[i] = p.sw + (int64_t)min(t * 128 + wn * 64 + i * 32 + r, p.N - 1) * p.ldsw; sw_next[i] = *(const uint32_t*)sp[i]; }
-  };
-  aim_scales(t0);
-  __syncthreads();
-  f32x16 acc[2];
-  const int xrow = wm * 32 + r;
-  const uint8_t* xr0 = xs + xrow * nkb * 128;
-  const uint8_t* wr0 = ws + (wn * 64 + r) * 128;
-  int off[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) off[c] = ((4 * h + c) ^ turn(r)) * 16;
-  int t = t0, kb = 0;
-  auto one = [&](int half, i32x4 (&next)[4]) __attribute__((always_inline)) {            // `next` holds the tile of the next step
-    if (kb == 0) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-    }
-    if ((kb & 3) == 0) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) sw_now[i] = sw_next[i];
-      if (kb + 4 < nkb) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) sw_next[i] = *(const uint32_t*)(sp[i] + kb + 4);
-      } else aim_scales(t + 1);
-    }
-    const int sa = se[xrow * LIN_NKB + kb];
-    const uint8_t *xr = xr0 + kb * 128, *wr = wr0 + half * 16384;
+template <int FA, int FB, int SA, int SB> __device__ inline f32x16 mfma8s(i32x8 a, i32x8 b, f32x16 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, SA, sa, SB, sb);
+}
+template <int FX, int NKB, int KB = 0> __device__ inline void lin_chain(f32x16& acc, const i32x8 (&w)[NKB][2], const uint32_t* sw, const uint32_t* sx, const uint8_t* x, const int (&off)[4]) {
+  if constexpr (KB < NKB) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
-      const i32x8 fx = __builtin_shufflevector(*(const i32x4*)(xr + off[2 * ks]), *(const i32x4*)(xr + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+      const uint8_t* t = x + KB * 64 * 128;
+      const i32x8 f = __builtin_shufflevector(*(const i32x4*)(t + off[2 * ks]), *(const i32x4*)(t + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+      acc = mfma8s<F8_E4M3, FX, KB & 3, KB & 3>(w[KB][ks], f, acc, (int)sw[KB / 4], (int)sx[KB / 4]);
+    }
+    lin_chain<FX, NKB, KB + 1>(acc, w, sw, sx, x, off);
+  }
+}
+
+template <int T, int FX, int NKB>
+__global__ __launch_bounds__(lin_threads<NKB>()) void k_fp8_linear(Fp8Linear p) {
+  constexpr int NT = lin_threads<NKB>(), NW = NT / 64, TASKS = 64 * NKB * 4, ROUNDS = (TASKS + NT - 1) / NT, WORDS = (NKB + 3) / 4;
+  __shared__ __attribute__((aligned(16))) uint8_t xs[2][NKB][64][128];         // 16-byte pieces turned by the row
+  __shared__ __attribute__((aligned(16))) uint8_t se[2][64][4 * WORDS];        // exponents + 127
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
+  // blocks b and b + 8 run on the same XCD: the parts of a row range go there and share its rows in that L2
+  const int xcd = blockIdx.x & 7, jj = blockIdx.x >> 3, part = jj % p.parts;
+  const int64_t lo = ((int64_t)(jj / p.parts) * 8 + xcd) * p.rows, hi = lo + p.rows < p.M ? lo + p.rows : p.M;
+  if (lo >= hi) return;
+  const int wn = wave % p.wn, wm = wave / p.wn, step = NW / p.wn, n0 = (part * p.wn + wn) * 32;
+  Eight<T> v[ROUNDS][4];
+  // (a uniform base and a 32-bit offset of the lane in bytes: pitches are under 2^25.  Rows behind the tile's last are read as that one: what is
+  // made of them is never stored.)
+  auto load = [&](int64_t m) __attribute__((always_inline)) {
+    const uint8_t* base = (const uint8_t*)p.x + 2 * m * p.ldx;
+    const int last = (int)(hi - m < p.bm ? hi - m : p.bm) - 1;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const i32x8 fw = __builtin_shufflevector(*(const i32x4*)(wr + i * 4096 + off[2 * ks]), *(const i32x4*)(wr + i * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
-        acc[i] = mfma8<F8_E4M3, FX>(fw, fx, acc[i], (int)sw_now[i], sa);
+    for (int q = 0; q < ROUNDS; ++q) {
+      const int task = tid + q * NT, l = task & 3, b = (task >> 2) % NKB, row = min((task >> 2) / NKB, last);
+      const uint32_t at = 2 * ((uint32_t)row * (uint32_t)p.ldx + b * 128 + l * 8);
+      if (p.K == NKB * 128) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) __builtin_memcpy(&v[q][j].v, base + at + 64 * j, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[q][j].load(base + at + 64 * j, 0, p.K - (b * 128 + (4 * j + l) * 8));
       }
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i) sw_now[i] >>= 8;
-    if (++kb == nkb) {
-      __syncthreads();          // every wave is done with this half of the tiles: it takes the result's turn
-      store_block<false>(p.o, acc[0], acc[1], ws + half * 16384 + wave * 4096, m0 + wm * 32, p.M, t * 128 + wn * 64, p.N, lane);
-      kb = 0; ++t;
-    }
-    stash(half ^ 1, next);
-    fetch(next);
-    __syncthreads();
   };
-  for (int step = 0; step < steps; step += 2) {
-    one(0, wb);
-    if (step + 1 < steps) one(1, wa);
+  auto cut = [&](int buf) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < ROUNDS; ++q) {
+      const int task = tid + q * NT, l = task & 3, b = (task >> 2) % NKB, row = (task >> 2) / NKB;
+      if (TASKS % NT != 0 && task >= TASKS) continue;
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { const uint32_t a = v[q][j].amax(); m = a > m ? a : m; }
+      const BlockScale bs = block_scale<FX>(dpp_umax<0x4E>(dpp_umax<0xB1>(m)));
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *(uint2*)&xs[buf][b][row][((2 * j + (l >> 1)) ^ turn(row)) * 16 + (l & 1) * 8] = quant8<T, FX>(v[q][j], bs);
+      if (l == 0) se[buf][row][b] = bs.byte;
+    }
+  };
+  load(lo);
+  i32x8 w[NKB][2];
+  uint32_t sw[WORDS];
+  {
+    const int n = min(n0 + r, p.N - 1);
+    const uint8_t* row = p.w + (int64_t)n * p.ldw + h * 64;
+#pragma unroll
+    for (int b = 0; b < NKB; ++b)
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks)
+        w[b][ks] = __builtin_shufflevector(*(const i32x4*)(row + b * 128 + ks * 32), *(const i32x4*)(row + b * 128 + ks * 32 + 16), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int b = 0; b < WORDS; ++b) sw[b] = *(const uint32_t*)(p.sw + (int64_t)n * p.ldsw + 4 * b);
+  }
+  cut(0);
+  if (lo + p.bm < hi) load(lo + p.bm);
+  __syncthreads();
+  int off[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) off[c] = r * 128 + ((4 * h + c) ^ turn(r)) * 16;
+  int buf = 0;
+  for (int64_t m = lo; m < hi; m += p.bm, buf ^= 1) {
+    const int rows = (int)(hi - m < p.bm ? hi - m : p.bm);
+    if (n0 < p.N)
+      for (int sub = wm; sub * 32 < rows; sub += step) {
+        f32x16 acc;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+        uint32_t sx[WORDS];
+#pragma unroll
+        for (int b = 0; b < WORDS; ++b) sx[b] = *(const uint32_t*)&se[buf][sub * 32 + r][4 * b];
+        lin_chain<FX, NKB>(acc, w, sw, sx, &xs[buf][0][sub * 32][0], off);
+        // lane = row r of y, register e = column 8 (e / 4) + 4 h + e % 4: two groups of eight columns trade halves between the halves of the
+        // wave, and every lane holds 16 bytes of its row
+#pragma unroll
+        for (int g = 0; g < 2; ++g) {
+          f32x4 a = {acc[8 * g], acc[8 * g + 1], acc[8 * g + 2], acc[8 * g + 3]}, b = {acc[8 * g + 4], acc[8 * g + 5], acc[8 * g + 6], acc[8 * g + 7]};
+          if (p.o.relu) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { a[j] = relu_nan(a[j]); b[j] = relu_nan(b[j]); }
+          }
+          typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+          u32x2 ua, ub;
+          if (p.o.type == FT_F16) { ua = __builtin_bit_cast(u32x2, __builtin_convertvector(a, h16x4)); ub = __builtin_bit_cast(u32x2, __builtin_convertvector(b, h16x4)); }
+          else { ua = __builtin_bit_cast(u32x2, __builtin_convertvector(a, b16x4)); ub = __builtin_bit_cast(u32x2, __builtin_convertvector(b, b16x4)); }
+          const auto s0 = __builtin_amdgcn_permlane32_swap(ua[0], ub[0], false, false), s1 = __builtin_amdgcn_permlane32_swap(ua[1], ub[1], false, false);
+          const i32x4 out = {(int)s0[0], (int)s1[0], (int)s0[1], (int)s1[1]};
+          const int n = n0 + 16 * g + 8 * h, row = sub * 32 + r;
+          if (row < rows && n < p.N) {
+            uint16_t* y = (uint16_t*)((uint8_t*)p.o.y + 2 * m * p.o.ldy + 2 * ((uint32_t)row * (uint32_t)p.o.ldy + (uint32_t)n));
+            if (n + 8 <= p.N) __builtin_memcpy(y, &out, 16);
+            else {
+#pragma unroll
+              for (int j = 0; j < 7; ++j) if (n + j < p.N) y[j] = (uint16_t)((uint32_t)out[j / 2] >> (16 * (j & 1)));
+            }
+          }
+        }
+      }
+    if (m + p.bm < hi) {
+      cut(buf ^ 1);
+      if (m + 2 * p.bm < hi) load(m + 2 * p.bm);
+    }
+    __syncthreads();            // this tile has been read, the next one is written
   }
 }
 
@@ -872,20 +874,30 @@ extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int3
   const int64_t nb = ceil128(K) / 128;
   return M * nb * 128 + up16(M * ((nb + 3) / 4 * 4)) + aln_fp8_nt_ws_bytes(M, N, K);
 }
-template <int T, int FX> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
-  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_linear<T, FX>, hipFuncAttributeMaxDynamicSharedMemorySize, lin_lds(LIN_NKB));
-  ALN_REQUIRE(big == hipSuccess, "fp8_linear: %s", hipGetErrorString(big));
-  const int64_t g = ((p.M + LIN_BM - 1) / LIN_BM + 7) / 8 * 8 * p.parts;
+template <int T, int FX, int NKB> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
+  const int64_t g = ((p.M + p.rows - 1) / p.rows + 7) / 8 * 8 * p.parts;
   ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_linear: %lld x %d results are too many for one launch", (long long)p.M, p.N);
-  hipLaunchKernelGGL((k_fp8_linear<T, FX>), dim3((uint32_t)g), dim3(256), lin_lds(p.nkb), st, p);
+  hipLaunchKernelGGL((k_fp8_linear<T, FX, NKB>), dim3((uint32_t)g), dim3(lin_threads<NKB>()), 0, st, p);
   ALN_CHECK_LAUNCH("fp8_linear");
   return 0;
+}
+template <int T, int FX> static int lin_pick(const Fp8Linear& p, int nkb, hipStream_t st) {
+  switch (nkb) {
+    case 1: return lin_launch<T, FX, 1>(p, st);
+    case 2: return lin_launch<T, FX, 2>(p, st);
+    case 3: return lin_launch<T, FX, 3>(p, st);
+    case 4: return lin_launch<T, FX, 4>(p, st);
+    case 5: return lin_launch<T, FX, 5>(p, st);
+    case 6: return lin_launch<T, FX, 6>(p, st);
+    case 7: return lin_launch<T, FX, 7>(p, st);
+    default: return lin_launch<T, FX, 8>(p, st);
+  }
 }
 extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, const void* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, int32_t fmt_w,
                               int64_t M, int32_t N, int32_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws, int64_t ws_bytes, void* stream) {
   ALN_REQUIRE(is_ft(x_type) && is_ft(y_type) && is_f8(fmt_x) && is_f8(fmt_w), "fp8_linear: unknown type %d, %d or format %d, %d", x_type, y_type, fmt_x, fmt_w);
-  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldx >= 0 && ldy >= N, "fp8_linear: sizes %lld x %d x %d, pitches %lld, %lld", (long long)M, N, K,
-              (long long)ldx, (long long)ldy);
+  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldx >= 0 && ldy >= N && ldx < 1 << 25 && ldy < 1 << 25,
+              "fp8_linear: sizes %lld x %d x %d, pitches %lld, %lld (under 2^25)", (long long)M, N, K, (long long)ldx, (long long)ldy);
   if (M == 0) return 0;
   ALN_REQUIRE(blocks_ok(w, ldw, sw, ldsw, K), FP8_BAD_BLOCKS, "fp8_linear");
   ALN_REQUIRE(x && ((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0 && y && ((uintptr_t)y & (y_type == FT_F32 ? 3 : 1)) == 0, "fp8_linear: x or y is NULL or not aligned to its type");
@@ -898,16 +910,21 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
     if (rc) return rc;
     return aln_fp8_nt(q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, fmt_x, w, ldw, sw, ldsw, fmt_w, M, N, K, y, ldy, y_type, relu, rest, ws_bytes - (rest - q), stream);
   }
-  // parts: the columns of y are cut only while the row tiles leave CUs without work (a part cuts the tile's rows into blocks again)
-  const int64_t mt = (M + LIN_BM - 1) / LIN_BM;
-  const int nt = (N + 127) / 128;
-  int parts = (int)(mt >= 512 ? 1 : 512 / mt);
-  if (parts > nt) parts = nt;
-  const int per = (nt + parts - 1) / parts;
-  const Fp8Linear p{x, ldx, (const uint8_t*)w, ldw, sw, ldsw, M, N, K, nkb, (nt + per - 1) / per, per, Fp8Out{y, ldy, y_type, relu}};
+  // One block of threads per CU.  While there are fewer 64-row tiles than CUs the columns of y are cut into more parts (each cuts the rows
+  // into blocks again); the rows then go round evenly, in tiles of one size.
+  const int waves = nkb <= 4 ? 16 : 8, need_wn = (N + 31) / 32;
+  const int64_t mt = (M + 63) / 64;
+  int wn = 1;
+  while (wn < waves && wn < need_wn && ((need_wn + wn - 1) / wn) * mt > 256) wn *= 2;
+  const int parts = (need_wn + wn - 1) / wn;
+  int64_t blocks = parts >= 256 ? 1 : 256 / parts;
+  if (blocks > mt) blocks = mt;
+  const int64_t rows = (M + blocks - 1) / blocks, tiles = (rows + 63) / 64;
+  ALN_REQUIRE(rows < (int64_t)1 << 31, "fp8_linear: too many rows");
+  const Fp8Linear p{x, ldx, (const uint8_t*)w, ldw, sw, ldsw, M, N, K, wn, parts, (int)rows, (int)((rows + tiles - 1) / tiles), Fp8Out{y, ldy, y_type, relu}};
   hipStream_t st = (hipStream_t)stream;
-  return x_type == FT_F16 ? (fmt_x == F8_E4M3 ? lin_launch<FT_F16, F8_E4M3>(p, st) : lin_launch<FT_F16, F8_E5M2>(p, st))
-                          : (fmt_x == F8_E4M3 ? lin_launch<FT_BF16, F8_E4M3>(p, st) : lin_launch<FT_BF16, F8_E5M2>(p, st));
+  return x_type == FT_F16 ? (fmt_x == F8_E4M3 ? lin_pick<FT_F16, F8_E4M3>(p, nkb, st) : lin_pick<FT_F16, F8_E5M2>(p, nkb, st))
+                          : (fmt_x == F8_E4M3 ? lin_pick<FT_BF16, F8_E4M3>(p, nkb, st) : lin_pick<FT_BF16, F8_E5M2>(p, nkb, st));
 }
 
 // ---- dW [N, K] (fp32, contiguous) = G^T X over M rows.  16-bit g and x of one type: the one-launch kernel (and the addition of its parts);

@@ -147,6 +147,8 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
     rows = _rows('linear', x)
     _need(rows.shape[1] == weight.cols, f'linear: x has {rows.shape[1]} columns, the weight {weight.cols}')
     out_dtype = _out_type('linear', out_dtype or x.dtype)
+    if rows.stride(0) >= 1 << 25:      # (rows very far apart)
+        rows = rows.detach().clone(memory_format=torch.contiguous_format)
     (m, k), n = rows.shape, weight.rows
     _need(n >= 1, 'linear: the weight has no rows')
     with _on(rows, weight.q):

@@ -467,7 +467,7 @@ int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t ldsa, int3
                int64_t ldsb, int32_t fmt_b, int64_t M, int32_t N, int64_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws,
                int64_t ws_bytes, void* stream);
 
-/* y [M, N] = x W^T for x [M, K] as it is (row pitch ldx): its rows are cut into blocks of fmt_x on the way -- the same result as
+/* y [M, N] = x W^T for x [M, K] as it is (row pitches ldx, ldy under 2^25 elements): its rows are cut into blocks of fmt_x on the way -- the same result as
  * aln_fp8_quantize + aln_fp8_nt up to the order of the fp32 additions.  ws: aln_fp8_linear_ws_bytes(same sizes and types) bytes, 16-byte aligned
  * (0: may be NULL). */
 int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t x_type, int32_t y_type, int32_t fmt_w);
