@@ -463,13 +463,19 @@ __global__ __launch_bounds__(lin_threads<NKB>()) void k_fp8_linear(Fp8Linear p) 
 #pragma unroll
     for (int q = 0; q < ROUNDS; ++q) {
       const int task = tid + q * NT, l = task & 3, b = (task >> 2) % NKB, row = min((task >> 2) / NKB, last);
-      const uint32_t at = 2 * ((uint32_t)row * (uint32_t)p.ldx + b * 128 + l * 8);
+      const uint32_t at = 2 * (uint32_t)row * (uint32_t)p.ldx;
+      const int k = b * 128 + l * 8;
       if (p.K == NKB * 128) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) __builtin_memcpy(&v[q][j].v, base + at + 64 * j, 16);
+        for (int j = 0; j < 4; ++j) __builtin_memcpy(&v[q][j].v, base + (at + 2 * k) + 64 * j, 16);
+      } else if (p.K % 8 == 0) {         // pieces behind the last column: read where the last one is, zero
+#pragma unroll
+        for (int j = 0; j < 4; ++j) __builtin_memcpy(&v[q][j].v, base + (at + 2 * min(k + 32 * j, p.K - 8)), 16);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) if (k + 32 * j >= p.K) v[q][j].v = (u16x8)(uint16_t)0;
       } else {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[q][j].load(base + at + 64 * j, 0, p.K - (b * 128 + (4 * j + l) * 8));
+        for (int j = 0; j < 4; ++j) v[q][j].load(base + (at + 2 * k) + 64 * j, 0, p.K - (k + 32 * j));
       }
     }
   };
