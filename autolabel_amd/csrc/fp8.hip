@@ -497,7 +497,8 @@ __global__ __launch_bounds__(lin_threads<NKB>()) void k_fp8_linear(Fp8Linear p) 
   load(lo);
   i32x8 w[NKB][2];
   uint32_t sw[WORDS];
-  {
+  const bool busy = n0 < p.N && wm * 32 < p.bm;           // (others only cut)
+  if (busy) {
     const int n = min(n0 + r, p.N - 1);
     const uint8_t* row = p.w + (int64_t)n * p.ldw + h * 64;
 #pragma unroll
@@ -517,7 +518,7 @@ __global__ __launch_bounds__(lin_threads<NKB>()) void k_fp8_linear(Fp8Linear p) 
   int buf = 0;
   for (int64_t m = lo; m < hi; m += p.bm, buf ^= 1) {
     const int rows = (int)(hi - m < p.bm ? hi - m : p.bm);
-    if (n0 < p.N)
+    if (busy)
       for (int sub = wm; sub * 32 < rows; sub += step) {
         f32x16 acc;
 #pragma unroll
@@ -625,7 +626,9 @@ template <int T, int FMT> __device__ inline void tn_quant(u16x8 (&v)[8], uint8_t
   if (rg == 0) { *(f32x4*)(scale + c8) = (f32x4){s[0], s[1], s[2], s[3]}; *(f32x4*)(scale + c8 + 4) = (f32x4){s[4], s[5], s[6], s[7]}; }
 }
 
-template <int T, int FG, int NI>
+// TAIL: the last step is not whole or its pieces would reach over the tensors' end; the code for that costs the others registers (630 us -> 660
+// at 2^19 rows x 512 x 512, where there is none).
+template <int T, int FG, int NI, bool TAIL>
 __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
   constexpr int TN = 64 * NI, TK = 256, COLS = TN + TK, STRIPS = COLS / 32;      // 8 < STRIPS <= 16
   extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];     // [2][COLS][128], then [2][COLS] powers of two
@@ -650,30 +653,43 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
   const int rg = lane & 15, c8 = (lane >> 4) * 8;
   auto load = [&](int64_t step, int strip) __attribute__((always_inline)) {
     if (step >= s1 || strip >= STRIPS) return;
-    // a uniform base and a 32-bit offset of the lane: no 64-bit arithmetic per lane
+    // a uniform base and a 32-bit offset of the lane (ld < 2^24): no 64-bit arithmetic per lane
     const bool isg = strip < TN / 32;
     const int64_t ld = isg ? p.ldg : p.ldx;
     const int C = isg ? p.N : p.K, col = isg ? n0 + strip * 32 : k0 + (strip - TN / 32) * 32;
     if (col >= C) return;                                 // (whole strips behind the last column: cut from what is there, never stored)
-    const uint16_t* base = (const uint16_t*)(isg ? p.g : p.x);
+    const uint16_t* base = (const uint16_t*)(isg ? p.g : p.x) + step * 128 * ld + col;
+    // Columns stand alone, so what a lane reads behind the last one does not matter as long as it is memory of the tensor: pieces that begin
+    // behind it read the last piece instead, and the last piece's seven values too many lie in the rows behind (ld >= C).
+    const int c = min(c8, (C - 1 - col) & ~7);
     const int64_t left = p.M - (step + 1) * 128;          // rows behind this step
-    if (left >= 0 && (col + 32 <= C || left * ld >= 7)) {
-      // Columns stand alone, so what a lane reads behind the last one does not matter as long as it is memory of the tensor: pieces that
-      // begin behind it read the last piece instead, and the last piece's seven values too many lie in the rows behind (ld >= C).
-      const uint32_t off = 2 * ((uint32_t)rg * (uint32_t)ld + (uint32_t)min(c8, (C - 1 - col) & ~7));       // bytes; ld < 2^26
+    if (!TAIL || (left >= 0 && (col + 32 <= C || left * ld >= 7))) {
+      const uint32_t off = 2 * ((uint32_t)rg * (uint32_t)ld + (uint32_t)c);       // bytes
 #pragma unroll
-      for (int i = 0; i < 8; ++i) __builtin_memcpy(&v[i], (const uint8_t*)(base + (step * 128 + i * 16) * ld + col) + off, 16);
-    } else {               // the tensor's end: every address held inside it, rows behind the last one zero
+      for (int i = 0; i < 8; ++i) __builtin_memcpy(&v[i], (const uint8_t*)(base + i * 16 * ld) + off, 16);
+    } else {
+      // the tensor's end: rows behind the last one read that one and become zero, a piece that would reach over the end begins earlier and
+      // is shifted down (the tensor has eight values or more)
+      const int last = (int)(p.M - 1 - step * 128 < 127 ? p.M - 1 - step * 128 : 127);
+      const int64_t size = (p.M - 1 - step * 128) * ld + C - col;
+      const int end = (int)(size < 0x7fffffff ? size : 0x7fffffff) - 8;            // where the last piece may begin (it may lie before the base)
+      int over[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int64_t row = step * 128 + rg + i * 16;
-        const uint16_t* at = base + min(row, p.M - 1) * ld;
-        uint16_t e[8];
+        const int at = min(rg + 16 * i, last) * (int)ld + c;
+        over[i] = at > end ? at - end : 0;
+        __builtin_memcpy(&v[i], base + (at - over[i]), 16);
+      }
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) e[j] = at[min(col + c8 + j, C - 1)];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = row < p.M ? e[j] : (uint16_t)0;
-        __builtin_amdgcn_sched_barrier(0);     // (a row at a time: eight loads in flight, not 64 with their addresses)
+      for (int i = 0; i < 8; ++i) {
+        typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+        u64x2 w = __builtin_bit_cast(u64x2, v[i]);
+        const int bits = 16 * over[i];
+        if (bits >= 64) { w[0] = w[1] >> (bits - 64); w[1] = 0; }
+        else if (bits > 0) { w[0] = (w[0] >> bits) | (w[1] << (64 - bits)); w[1] >>= bits; }
+        if (rg + 16 * i > last) w = (u64x2)0;
+        v[i] = __builtin_bit_cast(u16x8, w);
       }
     }
   };
@@ -687,12 +703,13 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
   };
   // Waves 4 .. 7 sit on the same SIMDs as 0 .. 3: with a lower priority they fall behind, and one of a pair multiplies while the other cuts.
   if (wave < 4) __builtin_amdgcn_s_setprio(1);
+  const bool busy = n0 + wn * 32 * NI < p.N && k0 + wk * 64 < p.K;      // (waves without results only cut)
   load(s0, wave);
   const int64_t halves = 2 * (s1 - s0 + 1);
   for (int64_t u = 0; u < halves; ++u) {     // two halves to a step: half of step s0 + u / 2 - 1 is multiplied, a strip of step s0 + u / 2 cut
     const int half = (int)u & 1;
     const int64_t next = s0 + (u >> 1);
-    if (u >= 2) {
+    if (u >= 2 && busy) {
       const int buf = (int)(next - 1 - s0) & 1;
       const uint8_t* gt = smem8 + (buf * COLS + wn * 32 * NI + r) * 128;
       const uint8_t* xt = smem8 + (buf * COLS + TN + wk * 64 + r) * 128;
@@ -729,16 +746,23 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
     load(next + half, wave + 8 - 8 * half);
     if (half) __syncthreads();            // the step has been read, the next one is written
   }
-  float* y = p.y + (int64_t)part * p.N * p.K;
+  // lane = column k, register e = row 8 (e / 4) + 4 h + e % 4 of a 32 x 32 block: a uniform row and a 32-bit offset of the lane
+  if (!busy || k0 + wk * 64 + r >= p.K) return;
+  const int nw = n0 + wn * 32 * NI;
+  float* y = p.y + ((int64_t)part * p.N + nw) * p.K + k0 + wk * 64;
+  const bool second = k0 + wk * 64 + 32 + r < p.K;
+  const uint32_t off = 4u * h * (uint32_t)p.K + r;        // (K < 2^24)
 #pragma unroll
   for (int i = 0; i < NI; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int n = n0 + wn * 32 * NI + 32 * i + 8 * (e / 4) + 4 * h + e % 4, k = k0 + wk * 64 + 32 * j + r;
-        if (n < p.N && k < p.K) y[(int64_t)n * p.K + k] = acc[i][j][e];
+    for (int e = 0; e < 16; ++e) {
+      const int n = 32 * i + 8 * (e / 4) + e % 4;         // + 4 h
+      if (nw + n + 4 * h < p.N) {
+        float* row = y + (int64_t)n * p.K;
+        row[off] = acc[i][0][e];
+        if (second) row[off + 32] = acc[i][1][e];
       }
+    }
 }
 
 // The slabs of a split contraction, added in a fixed order and rounded once.  Eight threads share four results (their slabs' sums meet through
@@ -933,52 +957,58 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
                           : (fmt_x == F8_E4M3 ? lin_pick<FT_BF16, F8_E4M3>(p, nkb, st) : lin_pick<FT_BF16, F8_E5M2>(p, nkb, st));
 }
 
-// ---- dW [N, K] (fp32, contiguous) = G^T X over M rows.  16-bit g and x of one type: the one-launch kernel (and the addition of its parts);
+// ---- dW [N, K] (fp32, contiguous) = G^T X over M rows.  16-bit g and x of one type (eight values each): the one-launch kernel (and the addition of its parts);
 // otherwise both transposed into blocks in the workspace, then the product.
-static bool tn_fused(int g_type, int x_type) { return g_type == x_type && g_type != FT_F32; }
+static bool tn_fused(int64_t M, int N, int K, int g_type, int x_type) { return g_type == x_type && g_type != FT_F32 && M * N >= 8 && M * K >= 8; }
 struct TnPlan { int ni, tn, tk, parts, per; };
 static TnPlan tn_plan(int64_t M, int N, int K) {
   TnPlan t;
-  t.ni = N > 128 ? 4 : 2;
+  // 256 x 256 results to a block cut every value of g and x half as often as 128 x 256 do, where there are blocks enough for every CU
+  t.ni = N > 128 && (N + 255) / 256 * (int64_t)((K + 255) / 256) * ((M + 127) / 128) >= 512 ? 4 : 2;
   t.tn = (N + 64 * t.ni - 1) / (64 * t.ni); t.tk = (K + 255) / 256;
   const int64_t tiles = (int64_t)t.tn * t.tk, steps = (M + 127) / 128;
   int64_t parts = tiles >= 256 ? 1 : 256 / tiles;         // one block per CU
-  if (parts > (steps + 3) / 4) parts = (steps + 3) / 4;   // four steps at least
+  // four steps at least, where the parts' slabs are more than small change
+  if (parts * N * K > 1 << 20 && parts > (steps + 3) / 4) parts = (steps + 3) / 4;
+  if (parts > steps) parts = steps;
   t.per = (int)((steps + parts - 1) / parts);
   t.parts = (int)((steps + t.per - 1) / t.per);
   return t;
 }
 extern "C" int64_t aln_fp8_grad_weight_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t g_type, int32_t x_type) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
-  if (tn_fused(g_type, x_type)) { const TnPlan t = tn_plan(M, N, K); return t.parts > 1 ? (int64_t)t.parts * N * K * 4 : 0; }
+  if (tn_fused(M, N, K, g_type, x_type)) { const TnPlan t = tn_plan(M, N, K); return t.parts > 1 ? (int64_t)t.parts * N * K * 4 : 0; }
   const int64_t nb = ceil128(M) / 128, per_row = nb * 128 + (nb + 3) / 4 * 4;
   return up16(((int64_t)N + K) * per_row) + 16 * 4 + aln_fp8_nt_ws_bytes(N, K, M);
 }
-template <int T, int FG, int NI> static int tn_launch(const Fp8TN& p, int parts, hipStream_t st) {
+template <int T, int FG, int NI, bool TAIL> static int tn_launch(const Fp8TN& p, int parts, hipStream_t st) {
   constexpr int COLS = 64 * NI + 256, LDS = 2 * COLS * 132;
-  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI, TAIL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_grad_weight: %s", hipGetErrorString(big));
   const int64_t g = (int64_t)(parts + 7) / 8 * 8 * p.tn * p.tk;
   ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_grad_weight: %d x %d results are too many for one launch", p.N, p.K);
-  hipLaunchKernelGGL((k_fp8_tn<T, FG, NI>), dim3((uint32_t)g), dim3(512), LDS, st, p);
+  hipLaunchKernelGGL((k_fp8_tn<T, FG, NI, TAIL>), dim3((uint32_t)g), dim3(512), LDS, st, p);
   ALN_CHECK_LAUNCH("fp8_grad_weight");
   return 0;
 }
+template <int T, int FG, int NI> static int tn_tail(const Fp8TN& p, int parts, hipStream_t st) {
+  return p.M % 128 || p.N % 32 || p.K % 32 ? tn_launch<T, FG, NI, true>(p, parts, st) : tn_launch<T, FG, NI, false>(p, parts, st);
+}
 template <int T> static int tn_pick(const Fp8TN& p, const TnPlan& t, int fmt_g, hipStream_t st) {
-  if (fmt_g == F8_E4M3) return t.ni == 4 ? tn_launch<T, F8_E4M3, 4>(p, t.parts, st) : tn_launch<T, F8_E4M3, 2>(p, t.parts, st);
-  return t.ni == 4 ? tn_launch<T, F8_E5M2, 4>(p, t.parts, st) : tn_launch<T, F8_E5M2, 2>(p, t.parts, st);
+  if (fmt_g == F8_E4M3) return t.ni == 4 ? tn_tail<T, F8_E4M3, 4>(p, t.parts, st) : tn_tail<T, F8_E4M3, 2>(p, t.parts, st);
+  return t.ni == 4 ? tn_tail<T, F8_E5M2, 4>(p, t.parts, st) : tn_tail<T, F8_E5M2, 2>(p, t.parts, st);
 }
 extern "C" int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, int32_t fmt_g, const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t N, int32_t K,
                                    float* dw, void* ws, int64_t ws_bytes, void* stream) {
   ALN_REQUIRE(is_ft(g_type) && is_ft(x_type) && is_f8(fmt_g), "fp8_grad_weight: unknown type %d, %d or format %d", g_type, x_type, fmt_g);
-  ALN_REQUIRE(M >= 1 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldg >= N && ldx >= K && ldg < 1 << 26 && ldx < 1 << 26,
-              "fp8_grad_weight: sizes %lld x %d x %d, pitches %lld, %lld (at least the columns, under 2^26)", (long long)M, N, K, (long long)ldg, (long long)ldx);
+  ALN_REQUIRE(M >= 1 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldg >= N && ldx >= K && ldg < 1 << 24 && ldx < 1 << 24,
+              "fp8_grad_weight: sizes %lld x %d x %d, pitches %lld, %lld (at least the columns, under 2^24)", (long long)M, N, K, (long long)ldg, (long long)ldx);
   ALN_REQUIRE(g && ((uintptr_t)g & (g_type == FT_F32 ? 3 : 1)) == 0 && x && ((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0 && dw && ((uintptr_t)dw & 3) == 0,
               "fp8_grad_weight: g, x or dw is NULL or not aligned to its type");
   const int64_t need = aln_fp8_grad_weight_ws_bytes(M, N, K, g_type, x_type);
   ALN_REQUIRE(ws_bytes >= need && (need == 0 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_grad_weight: the workspace needs %lld bytes, aligned to 16", (long long)need);
   hipStream_t st = (hipStream_t)stream;
-  if (!tn_fused(g_type, x_type)) {
+  if (!tn_fused(M, N, K, g_type, x_type)) {
     const int64_t nb = ceil128(M) / 128, ld = nb * 128, lds = (nb + 3) / 4 * 4;
     uint8_t *qg = (uint8_t*)ws, *qx = qg + N * ld, *sg = qx + K * ld, *sx = sg + up16(N * lds), *rest = sx + up16(K * lds);
     int rc = aln_fp8_quantize_t(g, g_type, ldg, M, N, fmt_g, qg, ld, sg, lds, stream);

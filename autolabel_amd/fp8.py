@@ -178,7 +178,7 @@ def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True)
         dx = linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt).reshape(x.shape)
     if need_dw:
         # (rows that overlap, as an expanded gradient's do, or lie very far apart)
-        gr, xr = (t if t.shape[0] <= 1 or t.shape[1] <= t.stride(0) < 1 << 26 else t.contiguous() for t in (gr, xr))
+        gr, xr = (t if t.shape[0] <= 1 or t.shape[1] <= t.stride(0) < 1 << 24 else t.clone(memory_format=torch.contiguous_format) for t in (gr, xr))
         with _on(gr, xr):
             (m, n), k = gr.shape, xr.shape[1]
             if m == 0:

@@ -475,7 +475,7 @@ int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, co
                    int32_t fmt_w, int64_t M, int32_t N, int32_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws,
                    int64_t ws_bytes, void* stream);
 
-/* dw [N, K] (fp32, contiguous, overwritten) = G^T X for g [M, N] and x [M, K] as they are (row pitches ldg >= N, ldx >= K, under 2^26), M >= 1: both are cut into
+/* dw [N, K] (fp32, contiguous, overwritten) = G^T X for g [M, N] and x [M, K] as they are (row pitches ldg >= N, ldx >= K, under 2^24), M >= 1: both are cut into
  * blocks of 128 rows per column, g in fmt_g, x in e4m3 -- the weight gradient of y = x W^T.  Bit-reproducible.  ws:
  * aln_fp8_grad_weight_ws_bytes(same sizes and types) bytes, 16-byte aligned (0: may be NULL). */
 int64_t aln_fp8_grad_weight_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t g_type, int32_t x_type);
