@@ -968,8 +968,8 @@ static TnPlan tn_plan(int64_t M, int N, int K) {
   t.tn = (N + 64 * t.ni - 1) / (64 * t.ni); t.tk = (K + 255) / 256;
   const int64_t tiles = (int64_t)t.tn * t.tk, steps = (M + 127) / 128;
   int64_t parts = tiles >= 256 ? 1 : 256 / tiles;         // one block per CU
-  // four steps at least, where the parts' slabs are more than small change
-  if (parts * N * K > 1 << 20 && parts > (steps + 3) / 4) parts = (steps + 3) / 4;
+  // two steps at least, where the parts' slabs are more than small change
+  if (parts * N * K > 1 << 20 && parts > (steps + 1) / 2) parts = (steps + 1) / 2;
   if (parts > steps) parts = steps;
   t.per = (int)((steps + parts - 1) / parts);
   t.parts = (int)((steps + t.per - 1) / t.per);
