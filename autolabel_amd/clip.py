@@ -34,6 +34,7 @@ def _dense(t):
 
 # Unbound methods mapped over the lists: a list of 60 small gradients costs more on the host than on the device.
 _T = torch.Tensor
+_PLAIN = {torch.Tensor, torch.nn.Parameter}
 _dtype = operator.attrgetter('dtype')
 
 
@@ -67,21 +68,22 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
         if len(out) != n:
             raise ValueError(f'{name}: {n} tensors, {len(out)} outputs')
     every = grads if out is None else grads + out
-    good = all(map(torch.is_tensor, every)) and all(map(_T.is_contiguous, every))
-    if good:
-        types, device = list(map(_dtype, grads)), list(map(_T.get_device, every))
-        good = device[0] >= 0 and device.count(device[0]) == len(every) and TYPES.keys() >= set(types)
-        good = good and (out is None or (list(map(_dtype, out)) == types and list(map(_T.size, out)) == list(map(_T.size, grads))))
-    if not good or loss_scale is not None or found_inf is not None:
+    codes = None                 # the tensors' types, where the quick checks already tell
+    if set(map(type, every)) <= _PLAIN and all(map(_T.is_contiguous, every)):
+        device, types = set(map(_T.get_device, every)), set(map(_dtype, every))
+        same = out is None or list(map(_T.size, out)) == list(map(_T.size, grads))
+        if len(device) == 1 and len(types) == 1 and min(device) >= 0 and types <= TYPES.keys() and same:
+            codes = array.array('i', (TYPES[types.pop()],)) * n
+    if codes is None or loss_scale is not None or found_inf is not None:
         _check(name, grads, out, loss_scale, found_inf)
-        types = list(map(_dtype, grads))
+        codes = array.array('i', [TYPES[t.dtype] for t in grads])
     dev = grads[0].device
     with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
         norm = torch.empty((), dtype=torch.float32, device=dev)
         ws = torch.empty(H.lib().aln_grad_clip_ws_bytes(n), dtype=torch.uint8, device=dev)
         g, o = array.array('Q', map(_T.data_ptr, grads)), None if out is None else array.array('Q', map(_T.data_ptr, out))
-        sizes, types = array.array('q', map(_T.numel, grads)), array.array('i', map(TYPES.__getitem__, types))
-        H.call('aln_grad_clip', n, g.buffer_info()[0], None if o is None else o.buffer_info()[0], sizes.buffer_info()[0], types.buffer_info()[0], max_norm,
+        sizes = array.array('q', map(_T.numel, grads))
+        H.call('aln_grad_clip', n, g.buffer_info()[0], None if o is None else o.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], max_norm,
                int(apply), loss_scale.data_ptr() if loss_scale is not None else None, norm.data_ptr(),
                found_inf.data_ptr() if found_inf is not None else None, ws.data_ptr(), ws.numel(), H.raw_stream())
     return norm

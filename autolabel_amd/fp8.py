@@ -141,23 +141,28 @@ def matmul(a, b, out_dtype=torch.float16, relu=False):
 def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
     """x [..., K] W^T for ``weight`` = Fp8Blocks of W [N, K] -> [..., N] of x's type (or ``out_dtype``); the rows of x are cut into blocks of
     ``fmt`` on the way.  ``relu``: negative results become 0."""
-    _need(isinstance(weight, Fp8Blocks), 'linear: weight must be Fp8Blocks (fp8.quantize)')
+    if not isinstance(weight, Fp8Blocks):
+        raise ValueError('linear: weight must be Fp8Blocks (fp8.quantize)')
     weight._check('linear: weight')
-    _need(fmt in FORMATS, f'linear: unknown 8-bit format {fmt!r} (one of {", ".join(FORMATS)})')
+    if fmt not in FORMATS:
+        raise ValueError(f'linear: unknown 8-bit format {fmt!r} (one of {", ".join(FORMATS)})')
     rows = _rows('linear', x)
-    _need(rows.shape[1] == weight.cols, f'linear: x has {rows.shape[1]} columns, the weight {weight.cols}')
-    out_dtype = _out_type('linear', out_dtype or x.dtype)
+    (m, k), (n, ldw) = rows.shape, weight.q.shape
+    if k != weight.cols or n < 1:
+        raise ValueError(f'linear: x has {k} columns, the weight {n} rows of {weight.cols} columns')
+    if out_dtype is None:
+        out_dtype = x.dtype
+    elif out_dtype not in TYPES:
+        raise ValueError(f'linear: results are fp16, bf16 or fp32, not {out_dtype}')
     if rows.stride(0) >= 1 << 25:      # (rows very far apart)
         rows = rows.detach().clone(memory_format=torch.contiguous_format)
-    (m, k), n = rows.shape, weight.rows
-    _need(n >= 1, 'linear: the weight has no rows')
     with _on(rows, weight.q):
         y = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
-        nbytes = H.lib().aln_fp8_linear_ws_bytes(m, n, k, TYPES[x.dtype], TYPES[out_dtype], FORMATS[weight.fmt][0])
+        x_type, y_type, fmt_w = TYPES[x.dtype], TYPES[out_dtype], FORMATS[weight.fmt][0]
+        nbytes = H.lib().aln_fp8_linear_ws_bytes(m, n, k, x_type, y_type, fmt_w)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-        H.call('aln_fp8_linear', _p(rows), TYPES[x.dtype], _pitch(rows), FORMATS[fmt][0], _p(weight.q), weight.q.shape[1], _p(weight.scale),
-               weight.scale.shape[1], FORMATS[weight.fmt][0], m, n, k, _p(y), n, TYPES[out_dtype], int(bool(relu)), _p(ws) if nbytes else None, nbytes,
-               H.raw_stream())
+        H.call('aln_fp8_linear', rows.data_ptr(), x_type, _pitch(rows), FORMATS[fmt][0], weight.q.data_ptr(), ldw, weight.scale.data_ptr(),
+               weight.scale.shape[1], fmt_w, m, n, k, y.data_ptr(), n, y_type, 1 if relu else 0, ws.data_ptr() if nbytes else None, nbytes, H.raw_stream())
     return y
 
 
@@ -165,29 +170,37 @@ def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True)
     """Gradients of y = x W^T (no activation) from ``g`` = dL/dy [..., N] and ``x`` [..., K]: (dL/dx of x's type, dL/dW [N, K] fp32), either
     one None where not needed.  ``weight_t`` = Fp8Blocks of W^T [K, N] (not read for dL/dW alone: may be None then).  g is cut into blocks of
     ``grad_fmt`` along N for dL/dx, g and x along their rows for dL/dW; the sums over the rows are taken in a fixed order."""
-    _need(grad_fmt in FORMATS, f'linear_backward: unknown 8-bit format {grad_fmt!r} (one of {", ".join(FORMATS)})')
+    if grad_fmt not in FORMATS:
+        raise ValueError(f'linear_backward: unknown 8-bit format {grad_fmt!r} (one of {", ".join(FORMATS)})')
     gr, xr = _rows('linear_backward: g', g), _rows('linear_backward: x', x)
-    _need(g.shape[:-1] == x.shape[:-1], f'linear_backward: g has the rows {tuple(g.shape[:-1])}, x {tuple(x.shape[:-1])}')
-    if need_dx:
-        _need(isinstance(weight_t, Fp8Blocks), 'linear_backward: weight_t must be Fp8Blocks (fp8.quantize of the transposed weight)')
-        weight_t._check('linear_backward: weight_t')
-        _need(weight_t.rows == xr.shape[1] and weight_t.cols == gr.shape[1],
-              f'linear_backward: weight_t is {weight_t.rows} x {weight_t.cols}, x has {xr.shape[1]} columns and g {gr.shape[1]}')
+    if g.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f'linear_backward: g has the rows {tuple(g.shape[:-1])}, x {tuple(x.shape[:-1])}')
+    (m, n), k = gr.shape, xr.shape[1]
     dx = dw = None
     if need_dx:
-        dx = linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt).reshape(x.shape)
+        if not isinstance(weight_t, Fp8Blocks):
+            raise ValueError('linear_backward: weight_t must be Fp8Blocks (fp8.quantize of the transposed weight)')
+        weight_t._check('linear_backward: weight_t')
+        if weight_t.rows != k or weight_t.cols != n:
+            raise ValueError(f'linear_backward: weight_t is {weight_t.rows} x {weight_t.cols}, x has {k} columns and g {n}')
+        dx = linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt)
+        if len(x.shape) != 2:
+            dx = dx.reshape(x.shape)
     if need_dw:
-        # (rows that overlap, as an expanded gradient's do, or lie very far apart)
-        gr, xr = (t if t.shape[0] <= 1 or t.shape[1] <= t.stride(0) < 1 << 24 else t.clone(memory_format=torch.contiguous_format) for t in (gr, xr))
+        if m > 1:       # (rows that overlap, as an expanded gradient's do, or lie very far apart)
+            if not n <= gr.stride(0) < 1 << 24:
+                gr = gr.detach().clone(memory_format=torch.contiguous_format)
+            if not k <= xr.stride(0) < 1 << 24:
+                xr = xr.detach().clone(memory_format=torch.contiguous_format)
         with _on(gr, xr):
-            (m, n), k = gr.shape, xr.shape[1]
             if m == 0:
-                return dx, torch.zeros(n, k, device=x.device)
-            dw = torch.empty(n, k, device=x.device)
-            nbytes = H.lib().aln_fp8_grad_weight_ws_bytes(m, n, k, TYPES[g.dtype], TYPES[x.dtype])
+                return dx, torch.zeros(n, k, dtype=torch.float32, device=x.device)
+            dw = torch.empty(n, k, dtype=torch.float32, device=x.device)
+            g_type, x_type = TYPES[g.dtype], TYPES[x.dtype]
+            nbytes = H.lib().aln_fp8_grad_weight_ws_bytes(m, n, k, g_type, x_type)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-            H.call('aln_fp8_grad_weight', _p(gr), TYPES[g.dtype], _pitch(gr), FORMATS[grad_fmt][0], _p(xr), TYPES[x.dtype], _pitch(xr), m, n, k,
-                   _p(dw), _p(ws) if nbytes else None, nbytes, H.raw_stream())
+            H.call('aln_fp8_grad_weight', gr.data_ptr(), g_type, _pitch(gr), FORMATS[grad_fmt][0], xr.data_ptr(), x_type, _pitch(xr), m, n, k,
+                   dw.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, H.raw_stream())
     return dx, dw
 
 
