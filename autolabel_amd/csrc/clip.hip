@@ -86,28 +86,40 @@ __global__ __launch_bounds__(256) void k_grad_sumsq(ClipList l, double* part) {
   if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
 
-template <int T> __device__ inline void scale_chunk(const void* g, void* o, int64_t lo, int64_t hi, float f) {
+// NT: what goes to another buffer passes the caches by, so that the gradients just squared are still there (36 -> 33 us for the 14.8 M
+// parameters of a field with 512-wide heads).
+template <int T, bool NT> __device__ inline void scale_chunk(const void* g, void* o, int64_t lo, int64_t hi, float f) {
+  typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+  typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
   int64_t i = lo + threadIdx.x * 8;
 #pragma unroll 4
   for (; i + 8 <= hi; i += 2048) {
     float v[8];
     load8<T>(g, i, v);
     if constexpr (T == FT_F32) {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= f;
-      __builtin_memcpy((float*)o + i, v, 32);
+      const f32x4u a = {v[0] * f, v[1] * f, v[2] * f, v[3] * f}, b = {v[4] * f, v[5] * f, v[6] * f, v[7] * f};
+      f32x4u* p = (f32x4u*)((float*)o + i);
+      if (NT) { __builtin_nontemporal_store(a, p); __builtin_nontemporal_store(b, p + 1); }
+      else { p[0] = a; p[1] = b; }
     } else {
-      u16x8 w;
+      u16x8u w;
 #pragma unroll
       for (int j = 0; j < 8; ++j) w[j] = T == FT_F16 ? __builtin_bit_cast(uint16_t, (h16)(v[j] * f)) : __builtin_bit_cast(uint16_t, (__bf16)(v[j] * f));
-      __builtin_memcpy((uint16_t*)o + i, &w, 16);
+      u16x8u* p = (u16x8u*)((uint16_t*)o + i);
+      if (NT) __builtin_nontemporal_store(w, p);
+      else *p = w;
     }
   }
   if (i < hi) for (; i < hi; ++i) store1<T>(o, i, load1<T>(g, i) * f);
 }
+template <int T> __device__ inline void scale_chunk(const void* g, void* o, int64_t lo, int64_t hi, float f) {
+  if (g == o) scale_chunk<T, false>(g, o, lo, hi, f);
+  else scale_chunk<T, true>(g, o, lo, hi, f);
+}
 __global__ __launch_bounds__(256) void k_grad_scale(ClipList l, ClipRule r, int apply, int in_place) {
   __shared__ double lds4[4];
   double s = 0.0;
+#pragma unroll 4
   for (int i = threadIdx.x; i < r.parts; i += 256) s += r.part[i];
   double norm = sqrt(block_sum_d(s, lds4));
   if (r.loss_scale) norm /= (double)*r.loss_scale;
@@ -119,7 +131,10 @@ __global__ __launch_bounds__(256) void k_grad_scale(ClipList l, ClipRule r, int 
     if (r.found_inf && !finite) *r.found_inf = 1;
   }
   if (!apply || (in_place && f == 1.f)) return;
-  for (int c = blockIdx.x; c < l.first[l.count]; c += gridDim.x) {
+  // backwards: what was squared last is the likeliest to be in the caches still
+  const int total = l.first[l.count], grid = gridDim.x;
+  for (int c = (total - 1) / grid * grid + (int)blockIdx.x; c >= 0; c -= grid) {
+    if (c >= total) continue;
     const int k = clip_find(l, c);
     const int64_t lo = (int64_t)(c - l.first[k]) * CLIP_CHUNK, hi = min(lo + CLIP_CHUNK, l.n[k]);
     if (l.type[k] == FT_F32) scale_chunk<FT_F32>(l.g[k], l.o[k], lo, hi, f);
