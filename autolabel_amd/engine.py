@@ -20,7 +20,14 @@ class TrainEngine:
     def __init__(self, pipe, lr=5e-3, betas=(0.9, 0.99), eps=1e-15, weight_decay_net=1e-6, rgb_weight=1.0, depth_weight=0.1,
                  semantic_weight=1.0, feature_weight=0.5, feature_loss=False, num_steps=128, upsample_steps=128,
                  scaler=None, process_group=None, overlap_comm=True, grad_payload='f16', fuse_grid_adam=True, shard_optimizer=False,
-                 shard_gather='table', exchange_at_world_1=False, direct_wire=True, level_group=4):
+                 shard_gather='table', exchange_at_world_1=False, direct_wire=True, level_group=4, max_grad_norm=None):
+        # the gradients' global norm (unscaled) is clipped to max_grad_norm between the backward pass and the optimizer (None: not at all)
+        if max_grad_norm is not None and not float(max_grad_norm) >= 0:
+            raise ValueError(f'TrainEngine: max_grad_norm = {max_grad_norm}')
+        if max_grad_norm is not None and shard_optimizer:
+            raise ValueError('TrainEngine: max_grad_norm needs every rank to hold the whole gradient (shard_optimizer leaves it 1 / world of the table\'s)')
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self.grad_norm = None    # fp32 scalar on the device: the norm of the last clipped step, before clipping
         self.pipe, self.P, self.L = pipe, pipe.P, pipe.L
         # hash-grid levels per scatter launch / gradient bucket of the overlapped exchange (level_groups).  Resolved ONCE, here: an explicit
         # argument wins; ALN_LEVEL_GROUP is only the default for level_group=None (re-reading the environment on every call let the
@@ -90,7 +97,8 @@ class TrainEngine:
         self.overlap_comm = self.dp and bool(overlap_comm)   # False: one collective after the backward pass
         # single GPU: the scatter's second phase holds the table's exact gradient sums in LDS and takes the Adam step for the table
         # itself (step()); with more ranks the gradient has to be averaged first, so it goes through P.grad and aln_adam_step
-        self.fuse_grid_adam = bool(fuse_grid_adam) and not self.dp and L.n_grid > 0 and int(L.enc.grid.n_features) == 2
+        # (and with clipping the table's gradient has to be there in full before anything is stepped)
+        self.fuse_grid_adam = bool(fuse_grid_adam) and not self.dp and L.n_grid > 0 and int(L.enc.grid.n_features) == 2 and self.max_grad_norm is None
         self.grad_payload = grad_payload     # 'f16': the hash-grid gradient crosses the wire as fp16 (parallel.allreduce_bucket)
         self.direct_wire = bool(direct_wire)  # ... written by the scatter itself instead of an fp32 table gradient + a packing pass (_wire_direct)
         self._comm = torch.cuda.Stream(device=dv) if self.dp else None
@@ -158,8 +166,9 @@ class TrainEngine:
 
     def _wire_direct(self):
         """True when the hash-grid scatter writes the fp16 payload of the exchange itself (aln_encode_bwd_binned_wire): data parallelism,
-        fp16 on the wire, replicated optimizer.  (The sharded optimizer stages padded shards and clears its source: parallel.reduce_scatter_bucket.)"""
-        return bool(self.dp and self.grad_payload == 'f16' and self.shard is None and self.L.n_grid > 0 and self.direct_wire)
+        fp16 on the wire, replicated optimizer.  (The sharded optimizer stages padded shards and clears its source: parallel.reduce_scatter_bucket;
+        clipping scales the fp32 gradient, not its halves.)"""
+        return bool(self.dp and self.grad_payload == 'f16' and self.shard is None and self.L.n_grid > 0 and self.direct_wire and self.max_grad_norm is None)
 
     def averaged_gradient(self):
         """The flat gradient after all_reduce_grads() as fp32 (a copy): P.grad, with the table's part taken from the fp16 payload when the
@@ -262,6 +271,13 @@ class TrainEngine:
                                     payload=self.grad_payload, scratch=self._wire_full() if direct else self._wire(self.L.n_grid), force=True,
                                     prepacked=direct)
 
+    def clip_gradients(self):
+        """Clip P.grad (averaged over the ranks by then: every rank finds the same norm) to max_grad_norm.  The gradients keep their loss scale;
+        a norm that is not finite raises the step's overflow flag, and the optimizer skips the step and backs the scale off."""
+        if self.max_grad_norm is not None:
+            from .clip import clip_grad_norm_
+            self.grad_norm = clip_grad_norm_(self.P.grad[:self.L.n_total], self.max_grad_norm, loss_scale=self.state_f[0:1], found_inf=self.state_i[2:3])
+
     def optimizer_step(self, step_dev=None, skip_grid=False):
         P, L, sc = self.P, self.L, self.scaler_cfg
         if self.shard is not None:
@@ -306,6 +322,7 @@ class TrainEngine:
         fuse = self.fuse_grid_adam
         out = self.forward_backward(batch, seed, step, noise, u, step_dev, grid_adam=fuse)
         self.all_reduce_grads()
+        self.clip_gradients()
         self.optimizer_step(step_dev, skip_grid=fuse)    # (advances the device step counter of a captured step: no separate increment launch)
         return out
 

@@ -73,7 +73,11 @@ class Trainer:
                  local_rank=0, world_size=1, device=None, mute=False, fp16=False, eval_interval=1, max_keep_ckpt=2,
                  workspace='workspace', best_mode='min', use_loss_as_metric=True, report_metric_at_train=False,
                  use_checkpoint='latest', use_tensorboardX=False, scheduler_update_every_step=False, fused=None,
-                 process_group=None, use_graph=True, device_data='auto', use_graph_dp=False, shard_optimizer=False, dp_level_group=4):
+                 process_group=None, use_graph=True, device_data='auto', use_graph_dp=False, shard_optimizer=False, dp_level_group=4, max_grad_norm=None):
+        # clip the gradients' global norm to this before every optimizer step (None: the reference's loop, unclipped)
+        self.max_grad_norm = max_grad_norm
+        if max_grad_norm is not None and shard_optimizer and world_size > 1:
+            raise ValueError('max_grad_norm and shard_optimizer: no rank holds the whole gradient')
         self.name, self.opt, self.mute, self.metrics = name, opt, mute, metrics
         self.dp_level_group = int(dp_level_group)   # data parallel: hash-grid levels per scatter launch / gradient bucket (TrainEngine.level_groups)
         self.local_rank, self.world_size, self.workspace = local_rank, world_size, workspace
@@ -151,7 +155,8 @@ class Trainer:
                                       num_steps=getattr(opt, 'num_steps', self.model.num_steps_default),
                                       upsample_steps=getattr(opt, 'upsample_steps', self.model.upsample_steps_default),
                                       process_group=self.process_group, shard_optimizer=self.shard_optimizer, level_group=self.dp_level_group,
-                                      shard_gather='master' if self.ema is not None else 'table')   # (the EMA reads the fp32 masters every step)
+                                      shard_gather='master' if self.ema is not None else 'table',   # (the EMA reads the fp32 masters every step)
+                                      max_grad_norm=self.max_grad_norm)
             if old is not None:   # same parameters on a new buffer: the Adam moments / loss scale / step counters carry over
                 self.engine.load_state_dict(old.state_dict())
             self._graph = None
@@ -328,6 +333,7 @@ class SimpleTrainer(Trainer):
                 with torch.autocast('cuda', enabled=self.fp16):
                     _, _, loss = self.train_step(data)
                 self.scaler.scale(loss).backward()
+                self._clip_gradients()
                 for opt in self.optimizers:
                     self.scaler.step(opt)
                 self.scaler.update()
@@ -337,6 +343,17 @@ class SimpleTrainer(Trainer):
         if self.ema is not None:
             self.ema.update()
         self._step_scheduler(loss)
+
+    def _clip_gradients(self):
+        """Generic loop: unscale the optimizers' gradients (GradScaler.step then does not again) and clip their global norm."""
+        if self.max_grad_norm is None:
+            return
+        from .clip import clip_grad_norm_
+        for opt in self.optimizers:
+            self.scaler.unscale_(opt)
+        grads = [p.grad for opt in self.optimizers for g in opt.param_groups for p in g['params'] if p.grad is not None]
+        if grads:
+            clip_grad_norm_(grads, self.max_grad_norm)
 
     def fused_step(self, data):
         eng = self._engine()
@@ -500,6 +517,7 @@ class InteractiveTrainer(SimpleTrainer):
             with torch.autocast('cuda', enabled=self.fp16):
                 _, _, loss = self.train_step(data)
             self.scaler.scale(loss).backward()
+            self._clip_gradients()
             self.scaler.step(self.optimizer)
             self.scaler.update()
         self.step += 1

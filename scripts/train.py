@@ -44,6 +44,7 @@ def read_args():
     parser.add_argument('--global-batch', type=int, default=0, help='data parallel: fixed global batch (overrides --batch-size)')
     parser.add_argument('--cuda-ray', action='store_true', help='occupancy-grid marching (the reference hard-codes cuda_ray=False)')
     parser.add_argument('--march-samples', type=int, default=96, help='sample rows per ray with --cuda-ray')
+    parser.add_argument('--max-grad-norm', type=float, default=None, help="clip the gradients' global norm before every optimizer step (the reference does not)")
     return parser.parse_args()
 
 
@@ -90,7 +91,7 @@ def main():
                             fp16=True, ema_decay=0.95, lr_scheduler=scheduler, scheduler_update_every_step=False, metrics=[],
                             use_checkpoint='latest', local_rank=rank, world_size=world, process_group=pg,
                             device_data=False if flags.host_data else ('auto' if not flags.device_data else True), use_graph_dp=flags.dp_graph,
-                            shard_optimizer=flags.shard_optimizer, dp_level_group=flags.dp_level_group)
+                            shard_optimizer=flags.shard_optimizer, dp_level_group=flags.dp_level_group, max_grad_norm=flags.max_grad_norm)
     if world > 1:   # replicas start identical (a resumed checkpoint is read by every rank; the broadcast also covers a fresh init)
         parallel.broadcast_parameters(model._ensure_device().P.flat, pg)
         model._shadow_version = None
