@@ -7,7 +7,7 @@ nothing is clipped; the products run on the block-scaled matrix instructions and
 
     w = fp8.quantize(weight)                 # [out, in], once
     y = fp8.linear(x, w, relu=True)          # x [..., in] fp16 / bf16 / fp32 -> [..., out]
-    dx, dw = fp8.linear_backward(g, x, fp8.quantize(weight.t()))
+    dx, dw = fp8.linear_backward(g, x, fp8.quantize(weight, transpose=True))
 
 ``Linear`` wraps the three for autograd.  Every call allocates its results and its scratch from torch's allocator and enqueues on the current
 stream of the tensors' device; nothing is kept between calls and nothing synchronises, so the calls can be captured into a graph.
@@ -138,9 +138,10 @@ def matmul(a, b, out_dtype=torch.float16, relu=False):
     return y
 
 
-def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
+def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
     """x [..., K] W^T for ``weight`` = Fp8Blocks of W [N, K] -> [..., N] of x's type (or ``out_dtype``); the rows of x are cut into blocks of
-    ``fmt`` on the way.  ``relu``: negative results become 0."""
+    ``fmt`` on the way.  ``relu``: negative results become 0.  ``out``: a contiguous tensor of the result's shape to write it into (its type
+    decides the result's); it must not overlap x."""
     if not isinstance(weight, Fp8Blocks):
         raise ValueError('linear: weight must be Fp8Blocks (fp8.quantize)')
     weight._check('linear: weight')
@@ -150,6 +151,10 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
     (m, k), (n, ldw) = rows.shape, weight.q.shape
     if k != weight.cols or n < 1:
         raise ValueError(f'linear: x has {k} columns, the weight {n} rows of {weight.cols} columns')
+    if out is not None:
+        if not torch.is_tensor(out) or out.shape != (*x.shape[:-1], n) or not out.is_contiguous() or out.get_device() != x.get_device() or out_dtype not in (None, out.dtype):
+            raise ValueError(f'linear: out must be a contiguous tensor of shape {(*x.shape[:-1], n)} beside x (of out_dtype, where given)')
+        out_dtype = out.dtype
     if out_dtype is None:
         out_dtype = x.dtype
     elif out_dtype not in TYPES:
@@ -157,7 +162,7 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3'):
     if rows.stride(0) >= 1 << 25:      # (rows very far apart)
         rows = rows.detach().clone(memory_format=torch.contiguous_format)
     with _on(rows, weight.q):
-        y = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device)
+        y = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device) if out is None else out
         x_type, y_type, fmt_w = TYPES[x.dtype], TYPES[out_dtype], FORMATS[weight.fmt][0]
         nbytes = H.lib().aln_fp8_linear_ws_bytes(m, n, k, x_type, y_type, fmt_w)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
@@ -217,7 +222,7 @@ class _LinearFunction(torch.autograd.Function):
     def backward(ctx, g):
         x, weight = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        dx, dw = linear_backward(g, x, quantize(weight.detach().t()) if need_dx else None, ctx.grad_fmt, need_dx, need_dw)
+        dx, dw = linear_backward(g, x, quantize(weight, transpose=True) if need_dx else None, ctx.grad_fmt, need_dx, need_dw)
         return dx, None if dw is None else dw.to(weight.dtype), None
 
 

@@ -14,6 +14,7 @@ import torch
 import torch.nn as nn
 
 from . import hip as H
+from .fp8 import Linear as Fp8Linear
 from .pipeline import HipPipeline, ModelLayout, Params, f16
 from .renderer import NeRFRenderer
 
@@ -84,6 +85,7 @@ class ALNetwork(NeRFRenderer):
         self.semantic_features = _Block(nets['semf'].n_params, geo_feat_dim, hidden_dim_semantic)
         self.semantic_out = _Block(nets['semo'].n_params, hidden_dim_semantic + geo_feat_dim, semantic_classes)
         self._P = self._pipe = None
+        self.semantic_fp8 = False
         self._seed = 0
         self._shadow_version = None
         self.reset_parameters()
@@ -94,6 +96,16 @@ class ALNetwork(NeRFRenderer):
         (reference=True) switches it on so their finest-level cells are hit exactly as during training."""
         self.tcnn_fma = bool(on)
         self._layout.enc.grid.pos_fma = int(self.tcnn_fma)
+
+    def set_semantic_fp8(self, on=True):
+        """Rendering and point queries run the two hidden layers' products of a wide feature head (hidden_dim_semantic over 128: LSeg) in 8-bit
+        blocks with a power of two per 128 values (autolabel_amd.fp8) instead of fp16 while gradients are off (torch.no_grad / inference_mode).
+        Training is not touched."""
+        if on and not self._layout.sem_wide:
+            raise ValueError('set_semantic_fp8: the semantic heads of this model are not wide (they run in one fused fp16 kernel)')
+        self.semantic_fp8 = bool(on)
+        if self._pipe is not None:
+            self._pipe.sem_fp8 = self.semantic_fp8
 
     def _get_encoder(self, encoding):
         if encoding == 'freq':
@@ -155,6 +167,7 @@ class ALNetwork(NeRFRenderer):
                     P.flat[a:b].copy_(p.data.reshape(-1))
                     p.data = P.flat[a:b]
             self._P, self._pipe = P, HipPipeline(self._layout, P, density_scale=float(self.density_scale), min_near=float(self.min_near))
+            self._pipe.sem_fp8 = self.semantic_fp8
             if self.cuda_ray:
                 from .pipeline import OccupancyGrid
                 self._pipe.occ = OccupancyGrid(p0.device, G=self.grid_size, max_steps=self.max_steps, samples=self.march_samples,
@@ -236,7 +249,7 @@ class ALNetwork(NeRFRenderer):
         so[:, 1:1 + L.G] = geo_features.to(f16)
         fs, os_ = L.nets['semf'], L.nets['semo']
         if L.sem_wide:     # LSeg-width heads: wide.hip GEMMs, inputs built inside the kernels
-            logits, feat, _ = pipe.wide_sem_fwd(so, n, lambda name, shp: torch.empty(shp, dtype=f16, device=dev))
+            logits, feat, _ = pipe.wide_sem_fwd(so, n, lambda name, shp: torch.empty(shp, dtype=f16, device=dev), fp8=pipe.sem_fp8)
             return logits[:, :L.C], feat[:, :L.D]
         fin = torch.empty(n, fs.in_pad, dtype=f16, device=dev)
         feat = torch.empty(n, fs.out_pad, dtype=f16, device=dev)
@@ -261,12 +274,14 @@ class ALNetwork(NeRFRenderer):
 
 class Autoencoder(nn.Module):
     """Feature-compression autoencoder used offline by scripts/compute_feature_maps.py (autolabel/models.py:268-294).
-    Out of the hot path: plain torch modules with the reference's layer sizes."""
+    Out of the hot path: plain torch modules with the reference's layer sizes.  ``fp8=True``: the layers' products, forward and backward, in 8-bit
+    blocks (autolabel_amd.fp8.Linear; the same parameters and state_dict)."""
 
-    def __init__(self, in_features, bottleneck):
+    def __init__(self, in_features, bottleneck, fp8=False):
         super().__init__()
-        self.encoder = nn.Sequential(nn.Linear(in_features, 128, bias=False), nn.ReLU(), nn.Linear(128, bottleneck, bias=False), nn.ReLU())
-        self.decoder = nn.Sequential(nn.Linear(bottleneck, 128, bias=False), nn.ReLU(), nn.Linear(128, in_features, bias=False))
+        linear = Fp8Linear if fp8 else (lambda i, o: nn.Linear(i, o, bias=False))
+        self.encoder = nn.Sequential(linear(in_features, 128), nn.ReLU(), linear(128, bottleneck), nn.ReLU())
+        self.decoder = nn.Sequential(linear(bottleneck, 128), nn.ReLU(), linear(128, in_features))
 
     def forward(self, x, p=0.1):
         code = self.encoder(x)

@@ -26,7 +26,7 @@ class _RenderFn(torch.autograd.Function):
         train = any(ctx.needs_input_grad[5:])  # (grad mode is off inside Function.forward)
         out, c = pipe.forward(rays_o, rays_d, norms, cfg['num_steps'], cfg['upsample_steps'], cfg['perturb'], train=train,
                               seed=cfg['seed'], step=cfg['step'], noise=cfg.get('noise'), u=cfg.get('u'), bg=cfg['bg'],
-                              march=cfg.get('march', False))
+                              march=cfg.get('march', False), sem_fp8=pipe.sem_fp8 and not cfg['grad'])
         ctx.model, ctx.c = model, (c if train else None)
         ctx.set_materialize_grads(False)  # unused outputs arrive as None: their heads then get grad None like in the reference
         keys = ['image', 'depth', 'semantic', 'semantic_features', 'depth_variance', 'coordinates_map', 'weights_sum']
@@ -116,7 +116,7 @@ class NeRFRenderer(nn.Module):
                 self.update_extra_state()   # never rendered through an empty bitfield
         cfg = dict(num_steps=int(num_steps if num_steps is not None else self.num_steps_default),
                    upsample_steps=int(upsample_steps if upsample_steps is not None else self.upsample_steps_default), march=bool(self.cuda_ray),
-                   perturb=bool(perturb), seed=int(self._seed if seed is None else seed), step=self._render_calls,
+                   perturb=bool(perturb), seed=int(self._seed if seed is None else seed), step=self._render_calls, grad=torch.is_grad_enabled(),
                    bg=1.0 if bg_color is None else float(bg_color), noise=noise, u=u)
         self._render_calls += 1
         f = lambda t: t.reshape(-1, t.shape[-1]).float().contiguous()

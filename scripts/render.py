@@ -22,6 +22,7 @@ def read_args():
     parser.add_argument('--model-dir', type=str, required=True)
     parser.add_argument('--max-depth', type=float, default=7.5)
     parser.add_argument('--out', type=str, required=True)
+    parser.add_argument('--fp8-features', action='store_true', help='a wide (LSeg) feature head: its hidden layers in 8-bit blocks instead of fp16')
     return parser.parse_args()
 
 
@@ -58,6 +59,8 @@ def main():
     kw = dict(cuda_ray=True, march_samples=getattr(params, 'march_samples', 96)) if getattr(params, 'cuda_ray', False) else {}
     model = model_utils.create_model(dataset.min_bounds, dataset.max_bounds, n_classes, params, **kw).cuda().eval()
     model_utils.load_checkpoint(model, os.path.join(flags.model_dir, 'checkpoints'))
+    if flags.fp8_features:
+        model.set_semantic_fp8()
     try:
         from skvideo.io.ffmpeg import FFmpegWriter
         writer = FFmpegWriter(flags.out, inputdict={'-framerate': f'{flags.fps}'},

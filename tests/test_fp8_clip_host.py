@@ -130,3 +130,28 @@ def test_workspace_sizes():
     assert L.aln_fp8_nt_ws_bytes(0, 5, 5) == 0 and L.aln_fp8_nt_ws_bytes(1 << 20, 512, 512) == 0
     assert L.aln_fp8_nt_ws_bytes(512, 512, 1 << 20) % (512 * 512 * 4) == 0 and L.aln_fp8_nt_ws_bytes(512, 512, 1 << 20) > 0
     assert L.aln_grad_clip_ws_bytes(1) == L.aln_grad_clip_ws_bytes(120) > 0 and L.aln_grad_clip_ws_bytes(121) == 2 * L.aln_grad_clip_ws_bytes(120)
+
+
+def test_engine_and_trainer_refusals():
+    from autolabel_amd.engine import TrainEngine
+    from autolabel_amd.trainer import Trainer
+    with pytest.raises(ValueError, match='max_grad_norm'):
+        TrainEngine(None, max_grad_norm=-1.0)
+    with pytest.raises(ValueError, match='max_grad_norm'):
+        TrainEngine(None, max_grad_norm=math.nan)
+    with pytest.raises(ValueError, match='shard_optimizer'):
+        TrainEngine(None, max_grad_norm=1.0, shard_optimizer=True)
+    with pytest.raises(ValueError, match='shard_optimizer'):
+        Trainer('x', None, None, max_grad_norm=1.0, shard_optimizer=True, world_size=2)
+
+
+def test_autoencoder_keeps_its_parameters():
+    from autolabel_amd.models import Autoencoder
+    torch.manual_seed(0)
+    a = Autoencoder(32, 8)
+    torch.manual_seed(0)
+    b = Autoencoder(32, 8, fp8=True)
+    assert list(a.state_dict()) == list(b.state_dict())
+    assert all(torch.equal(x, y) for x, y in zip(a.state_dict().values(), b.state_dict().values()))
+    with pytest.raises(ValueError, match='no CPU path'):
+        b(torch.zeros(2, 32))
