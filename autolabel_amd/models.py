@@ -98,9 +98,9 @@ class ALNetwork(NeRFRenderer):
         self._layout.enc.grid.pos_fma = int(self.tcnn_fma)
 
     def set_semantic_fp8(self, on=True):
-        """Rendering and point queries run the two hidden layers' products of a wide feature head (hidden_dim_semantic over 128: LSeg) in 8-bit
-        blocks with a power of two per 128 values (autolabel_amd.fp8) instead of fp16 while gradients are off (torch.no_grad / inference_mode).
-        Training is not touched."""
+        """Rendering and point queries run the last layer's product of a wide feature head (hidden_dim_semantic over 128: LSeg) in 8-bit blocks with
+        a power of two per 128 values (autolabel_amd.fp8) instead of fp16 while gradients are off (torch.no_grad / inference_mode).  Training is
+        not touched."""
         if on and not self._layout.sem_wide:
             raise ValueError('set_semantic_fp8: the semantic heads of this model are not wide (they run in one fused fp16 kernel)')
         self.semantic_fp8 = bool(on)

@@ -275,7 +275,7 @@ class HipPipeline:
         # recompute kernel; other shapes (e.g. 64-wide density / color nets) save them and use the generic backward kernels
         self.recompute = all(k in params.wide_w or H.lib().aln_mlp_has_recompute(s.in_pad, s.hidden, s.out_pad, s.n_hidden)
                              for k, s in layout.nets.items())
-        self.sem_fp8 = False    # rendering without gradients / point queries: the wide feature head's hidden layers in 8-bit blocks (ALNetwork.set_semantic_fp8)
+        self.sem_fp8 = False    # rendering without gradients / point queries: the wide feature head's last layer in 8-bit blocks (ALNetwork.set_semantic_fp8)
         self.occ = None     # OccupancyGrid: forward(..., march=True) then places the samples by marching (enable_marching)
         self.kernel_events = None  # bench.py: list of ((start, end) HIP events, kernel, tag) around the timed launches
 
@@ -399,8 +399,9 @@ class HipPipeline:
     def wide_sem_fwd(self, sout, M, bufs, fp8=False):
         """f = semantic_features([geo, 1]); logits = semantic_out([relu(f), geo, 1]) for M rows of the density head's output.
         bufs: callable name, shape -> fp16 buffer.  Returns (logits [M, Cpad], f [M, D], saved activations).
-        ``fp8`` (inference): the products of semantic_features' two square layers in 8-bit blocks.  Their weights are cut into blocks here, at every
-        call (two launches over half a megabyte): a replayed training step changes them without telling anyone."""
+        ``fp8`` (inference): the product of semantic_features' last layer in 8-bit blocks (2^20 rows x 512 x 512: 0.50 ms against 0.83; the two layers
+        before it stay with the kernel that generates the first, which 8-bit layers of their own would not beat).  The weight is cut into blocks
+        here, at every call (one launch over half a megabyte): a replayed training step changes it without telling anyone."""
         L = self.L
         fs, os_ = L.nets['semf'], L.nets['semo']
         Wf, Wo = self.P.wide_w['semf'], self.P.wide_w['semo']
@@ -408,17 +409,15 @@ class HipPipeline:
         h2 = bufs('wide_h2', (M, fs.hidden))
         feat, ho = bufs('feat', (M, fs.out_pad)), bufs('wide_ho', (M, os_.hidden))
         logits = bufs('logits', (M, os_.out_pad))
-        if self._gen() and not fp8:    # layers 1 + 2 in one launch, h1 never stored
+        if self._gen():    # layers 1 + 2 in one launch, h1 never stored
             h1 = None
             self._nt_gen(M, h2, sout, tag=fl)
         else:
             h1 = bufs('wide_h1', (M, fs.hidden))
             self._nt(M, fs.hidden, Wf[0], h1, geo=sout, relu=1, tag=fl)
-            if not fp8:
-                self._nt(M, fs.hidden, Wf[1], h2, a1=h1, K1=fs.hidden, relu=1, tag=fl)
+            self._nt(M, fs.hidden, Wf[1], h2, a1=h1, K1=fs.hidden, relu=1, tag=fl)
         if fp8:
             from . import fp8 as F8
-            F8.linear(h1, F8.quantize(Wf[1]), relu=True, out=h2)
             F8.linear(h2, F8.quantize(Wf[2]), out=feat)
         else:
             self._nt(M, fs.out_pad, Wf[2], feat, a1=h2, K1=fs.hidden, tag=fl)
@@ -522,7 +521,7 @@ class HipPipeline:
         logits carry no loss, so semantic_out is skipped, and the last layer of semantic_features -- linear, no activation -- is
         applied ONCE PER RAY to the composited hidden activation instead of once per sample: sum_s w_s (W3 h2_s) = W3 (sum_s w_s h2_s)
         (autolabel/models.py:123, 248-256).  out['semantic'] is then zeros.
-        ``sem_fp8`` (no backward pass may follow): the wide feature head's hidden layers in 8-bit blocks (wide_sem_fwd)."""
+        ``sem_fp8`` (no backward pass may follow): the wide feature head's last layer in 8-bit blocks (wide_sem_fwd)."""
         L, P = self.L, self.P
         ws = self.ws if ws is None else ws     # (the training engine passes its own: see Workspace)
         N = rays_o.shape[0]

@@ -22,7 +22,7 @@ def read_args():
     parser.add_argument('--model-dir', type=str, required=True)
     parser.add_argument('--max-depth', type=float, default=7.5)
     parser.add_argument('--out', type=str, required=True)
-    parser.add_argument('--fp8-features', action='store_true', help='a wide (LSeg) feature head: its hidden layers in 8-bit blocks instead of fp16')
+    parser.add_argument('--fp8-features', action='store_true', help='a wide (LSeg) feature head: its last layer in 8-bit blocks instead of fp16')
     return parser.parse_args()
 
 
