@@ -13,6 +13,7 @@ nothing is clipped; the products run on the block-scaled matrix instructions and
 stream of the tensors' device; nothing is kept between calls and nothing synchronises, so the calls can be captured into a graph.
 """
 import contextlib
+import functools
 from dataclasses import dataclass
 
 import torch
@@ -51,9 +52,11 @@ class Fp8Blocks:
             raise ValueError(f'{name}: unknown 8-bit format {self.fmt!r} (one of {", ".join(FORMATS)})')
         nb = _blocks(self.cols)
         q, s = self.q, self.scale
-        if self.cols < 1 or q.dim() != 2 or q.dtype != FORMATS[self.fmt][1] or not q.is_contiguous() or q.shape[1] < nb * BLOCK or q.shape[1] % 16:
+        shape = q.shape
+        if self.cols < 1 or len(shape) != 2 or q.dtype is not FORMATS[self.fmt][1] or not q.is_contiguous() or shape[1] < nb * BLOCK or shape[1] % 16:
             raise ValueError(f'{name}: q must be contiguous {FORMATS[self.fmt][1]} [rows, whole blocks of 128 for {self.cols} columns], got {q.dtype} {tuple(q.shape)}')
-        if s.dim() != 2 or s.dtype != torch.uint8 or not s.is_contiguous() or s.shape[0] != q.shape[0] or s.shape[1] < nb or s.shape[1] % 4 or s.get_device() != q.get_device():
+        words = s.shape
+        if len(words) != 2 or s.dtype is not torch.uint8 or not s.is_contiguous() or words[0] != shape[0] or words[1] < nb or words[1] % 4 or s.get_device() != q.get_device():
             raise ValueError(f'{name}: scale must be contiguous uint8 [rows, a multiple of 4 >= {nb}] beside q, got {s.dtype} {tuple(s.shape)}')
 
 
@@ -91,6 +94,17 @@ def _on(a, b=None):
             raise ValueError('autolabel_amd.fp8 has no CPU path: needs device tensors')
         raise ValueError(f'tensors on different devices: {a.device} and {b.device}')
     return _NOTHING if i == torch.cuda.current_device() else torch.cuda.device(i)
+
+
+# (functions of the sizes alone)
+@functools.lru_cache(maxsize=4096)
+def _linear_ws_bytes(*sizes):
+    return H.lib().aln_fp8_linear_ws_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=4096)
+def _grad_weight_ws_bytes(*sizes):
+    return H.lib().aln_fp8_grad_weight_ws_bytes(*sizes)
 
 
 def _p(t):
@@ -164,7 +178,7 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
     with _on(rows, weight.q):
         y = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device) if out is None else out
         x_type, y_type, fmt_w = TYPES[x.dtype], TYPES[out_dtype], FORMATS[weight.fmt][0]
-        nbytes = H.lib().aln_fp8_linear_ws_bytes(m, n, k, x_type, y_type, fmt_w)
+        nbytes = _linear_ws_bytes(m, n, k, x_type, y_type, fmt_w)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         H.call('aln_fp8_linear', rows.data_ptr(), x_type, _pitch(rows), FORMATS[fmt][0], weight.q.data_ptr(), ldw, weight.scale.data_ptr(),
                weight.scale.shape[1], fmt_w, m, n, k, y.data_ptr(), n, y_type, 1 if relu else 0, ws.data_ptr() if nbytes else None, nbytes, H.raw_stream())
@@ -202,7 +216,7 @@ def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True)
                 return dx, torch.zeros(n, k, dtype=torch.float32, device=x.device)
             dw = torch.empty(n, k, dtype=torch.float32, device=x.device)
             g_type, x_type = TYPES[g.dtype], TYPES[x.dtype]
-            nbytes = H.lib().aln_fp8_grad_weight_ws_bytes(m, n, k, g_type, x_type)
+            nbytes = _grad_weight_ws_bytes(m, n, k, g_type, x_type)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
             H.call('aln_fp8_grad_weight', gr.data_ptr(), g_type, _pitch(gr), FORMATS[grad_fmt][0], xr.data_ptr(), x_type, _pitch(xr), m, n, k,
                    dw.data_ptr(), ws.data_ptr() if nbytes else None, nbytes, H.raw_stream())
