@@ -425,7 +425,6 @@ struct Fp8Linear {
   int rows, bm;                   // rows of a block of threads, of a tile (<= 64)
   Fp8Out o;
 };
-#define LIN_NKB 8
 template <int NKB> constexpr int lin_threads() { return NKB <= 4 ? 1024 : 512; }
 
 template <int FA, int FB, int SA, int SB> __device__ inline f32x16 mfma8s(i32x8 a, i32x8 b, f32x16 c, int sa, int sb) {
@@ -811,7 +810,7 @@ static int quant_launch(bool t, const void* x, int64_t ldx, int64_t M, int K, vo
     hipLaunchKernelGGL((k_fp8_quant<T, FMT>), dim3(aln_grid_for(M * nb, 16, 256 * 16)), dim3(256), 0, st, x, ldx, M, K, nb, (uint8_t*)q, ldq, scale, lds);
   } else {
     const int64_t nb = ceil128(M) / 128, g = nb * ((K + 63) / 64);
-    ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_quantize: %lld x %d values are too many for one launch", (long long)M, K);
+    ALN_REQUIRE(g < (int64_t)1 << 24, "fp8_quantize: %lld x %d values are too many for one launch", (long long)M, K);
     hipLaunchKernelGGL((k_fp8_quant_t<T, FMT>), dim3((uint32_t)g), dim3(256), 0, st, x, ldx, M, K, (int)nb, (uint8_t*)q, ldq, scale, lds);
   }
   ALN_CHECK_LAUNCH("fp8_quantize");
@@ -861,7 +860,7 @@ template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI> static int 
   static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_nt: %s", hipGetErrorString(big));
   const int64_t g = ((p.M + BM - 1) / BM + 7) / 8 * 8 * ((p.N + BN - 1) / BN);
-  ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_nt: %lld x %d results are too many for one launch", (long long)p.M, p.N);
+  ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_nt: %lld x %d results are too many for one launch", (long long)p.M, p.N);
   hipLaunchKernelGGL((k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>), dim3((uint32_t)g, p.splits), dim3(64 * WM * WN), LDS, st, p);
   ALN_CHECK_LAUNCH("fp8_nt");
   return 0;
@@ -895,18 +894,22 @@ extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t
   return 0;
 }
 
-// ---- x W^T for x as it is.  Up to 1024 columns, 16-bit x and y, e4m3 weights: the one-launch kernel; otherwise blocks of x in the workspace,
-// then the product.
-static bool lin_fused(int64_t K, int x_type, int y_type, int fmt_w) { return ceil128(K) / 128 <= LIN_NKB && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3; }
+// ---- x W^T for x as it is.  16-bit x and y, e4m3 weights, up to 512 columns (1024 with few columns of y): the one-launch kernel; otherwise blocks of
+// x in the workspace, then the product.
+// (eight waves hold 256 columns of y at 513 .. 1024 columns of x, and every further part cuts the rows again: 4096 x 768 x 768 takes 12.8 us, 14.9 in
+// two launches, but 8192 x 1024 x 1024 27.2, 25.3 in two, and 8192 x 1024 x 4096 65.8, 49.5 in two; up to 512 columns 131072 x 512 x 4096 482, 557 in two)
+static bool lin_fused(int N, int64_t K, int x_type, int y_type, int fmt_w) {
+  return (K <= 512 || (K <= 1024 && N <= 768)) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
+}
 static inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t x_type, int32_t y_type, int32_t fmt_w) {
-  if (M <= 0 || N <= 0 || K <= 0 || lin_fused(K, x_type, y_type, fmt_w)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || lin_fused(N, K, x_type, y_type, fmt_w)) return 0;
   const int64_t nb = ceil128(K) / 128;
   return M * nb * 128 + up16(M * ((nb + 3) / 4 * 4)) + aln_fp8_nt_ws_bytes(M, N, K);
 }
 template <int T, int FX, int NKB> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
   const int64_t g = ((p.M + p.rows - 1) / p.rows + 7) / 8 * 8 * p.parts;
-  ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_linear: %lld x %d results are too many for one launch", (long long)p.M, p.N);
+  ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_linear: %lld x %d results are too many for one launch", (long long)p.M, p.N);
   hipLaunchKernelGGL((k_fp8_linear<T, FX, NKB>), dim3((uint32_t)g), dim3(lin_threads<NKB>()), 0, st, p);
   ALN_CHECK_LAUNCH("fp8_linear");
   return 0;
@@ -934,7 +937,7 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
   const int64_t need = aln_fp8_linear_ws_bytes(M, N, K, x_type, y_type, fmt_w);
   ALN_REQUIRE(ws_bytes >= need && (need == 0 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_linear: the workspace needs %lld bytes, aligned to 16", (long long)need);
   const int nkb = (int)(ceil128(K) / 128);
-  if (!lin_fused(K, x_type, y_type, fmt_w)) {
+  if (!lin_fused(N, K, x_type, y_type, fmt_w)) {
     uint8_t* q = (uint8_t*)ws, *sc = q + M * nkb * 128, *rest = sc + up16(M * ((nkb + 3) / 4 * 4));
     const int rc = aln_fp8_quantize(x, x_type, ldx, M, K, fmt_x, q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, stream);
     if (rc) return rc;
@@ -986,7 +989,7 @@ template <int T, int FG, int NI, bool TAIL> static int tn_launch(const Fp8TN& p,
   static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI, TAIL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_grad_weight: %s", hipGetErrorString(big));
   const int64_t g = (int64_t)(parts + 7) / 8 * 8 * p.tn * p.tk;
-  ALN_REQUIRE(g < (int64_t)1 << 31, "fp8_grad_weight: %d x %d results are too many for one launch", p.N, p.K);
+  ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_grad_weight: %d x %d results are too many for one launch", p.N, p.K);
   hipLaunchKernelGGL((k_fp8_tn<T, FG, NI, TAIL>), dim3((uint32_t)g), dim3(512), LDS, st, p);
   ALN_CHECK_LAUNCH("fp8_grad_weight");
   return 0;

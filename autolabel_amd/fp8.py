@@ -175,6 +175,8 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
         raise ValueError(f'linear: results are fp16, bf16 or fp32, not {out_dtype}')
     if rows.stride(0) >= 1 << 25:      # (rows very far apart)
         rows = rows.detach().clone(memory_format=torch.contiguous_format)
+    if out is not None and m and rows.data_ptr() < out.data_ptr() + out.nbytes and out.data_ptr() < rows.data_ptr() + ((m - 1) * rows.stride(0) + k) * rows.element_size():
+        raise ValueError('linear: out must not overlap x')
     with _on(rows, weight.q):
         y = torch.empty(*x.shape[:-1], n, dtype=out_dtype, device=x.device) if out is None else out
         x_type, y_type, fmt_w = TYPES[x.dtype], TYPES[out_dtype], FORMATS[weight.fmt][0]

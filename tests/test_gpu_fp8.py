@@ -151,7 +151,8 @@ def test_matmul_formats_and_types(fp8, fa, fb, dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 512, 512), (2, 128, 3), (31, 129, 33), (64, 512, 512), (65, 528, 64), (128, 16, 16), (200, 640, 130), (257, 512, 300),
-          (5, 4096, 40), (3, 1030, 1000), (300, 1536, 96), (1000, 77, 130), (129, 2048, 257)]
+          (5, 4096, 40), (3, 1030, 1000), (300, 1536, 96), (1000, 77, 130), (129, 2048, 257), (70, 700, 200), (33, 893, 70), (130, 1000, 768),
+          (65, 1024, 1024), (1, 300, 1500), (70, 384, 1500), (9, 250, 2000), (700, 256, 31)]
 
 
 @pytest.mark.parametrize('relu', [False, True])
@@ -193,6 +194,72 @@ def test_linear_shapes_views_and_empty(fp8):
     assert fp8.linear(torch.empty(3, 0, 40, device='cuda'), wq).shape == (3, 0, 20)
     one = fp8.linear(x[0, 0, :40].cuda(), wq)          # a vector
     assert one.shape == (20,)
+
+
+@pytest.mark.parametrize('fx', ['e4m3', 'e5m2'])
+@pytest.mark.parametrize('fw', ['e4m3', 'e5m2'])
+@pytest.mark.parametrize('K', [200, 600, 1200])
+def test_linear_formats(fp8, fx, fw, K):
+    g = torch.Generator().manual_seed(K)
+    x, w = torch.randn(150, K, generator=g).bfloat16(), torch.randn(90, K, generator=g) / math.sqrt(K)
+    want, tol = product_bound(blocks64(x, fx)[0], blocks64(w, fw)[0], K, torch.bfloat16)
+    check(fp8.linear(x.cuda(), fp8.quantize(w.cuda(), fw), fmt=fx), want, tol)
+
+
+def test_linear_out(fp8):
+    x, wq = torch.randn(7, 30, 96, device='cuda').half(), fp8.quantize(torch.randn(40, 96, device='cuda'))
+    want = fp8.linear(x, wq)
+    out = torch.full((9, 30, 40), 7.0, device='cuda', dtype=torch.float16)
+    got = fp8.linear(x, wq, out=out[1:8])
+    assert got.data_ptr() == out[1:8].data_ptr() and torch.equal(out[1:8], want)
+    assert (out[0] == 7).all() and (out[8] == 7).all()           # what lies beside is left as it was
+    out32 = torch.empty(7, 30, 40, device='cuda')
+    assert torch.equal(fp8.linear(x, wq, out=out32), fp8.linear(x, wq, out_dtype=torch.float32))
+    for bad in (out[:6], out[1:8].transpose(0, 1), torch.empty(7, 30, 40)):
+        with pytest.raises(ValueError, match='out must be'):
+            fp8.linear(x, wq, out=bad)
+    with pytest.raises(ValueError, match='out must be'):
+        fp8.linear(x, wq, out=out32, out_dtype=torch.float16)
+    sq = fp8.quantize(torch.randn(96, 96, device='cuda'))
+    with pytest.raises(ValueError, match='overlap'):
+        fp8.linear(x, sq, out=x)
+
+
+@pytest.mark.parametrize('M,K,N', [(129, 1, 1), (256, 3, 5), (128, 7, 1), (135, 2, 9), (383, 8, 8), (4096, 40, 1), (8, 1, 1), (7, 1, 1), (1, 8, 8), (1, 3, 4),
+                                   (66000, 300, 300), (65536, 264, 520), (640, 30, 400)])
+def test_weight_gradient_edges(fp8, M, K, N):
+    """Where a piece of eight columns would reach over the tensors' end: both stand alone at the end of their memory here (a pool's block is larger,
+    but what lies behind is NaN, and must not be met)."""
+    r = torch.Generator().manual_seed(M + K + N)
+    x, gy = torch.randn(M, K, generator=r).half(), (torch.randn(M, N, generator=r) * 0.1).half()
+    xd, gd = torch.full((M * K + 64,), math.nan, device='cuda').half(), torch.full((M * N + 64,), math.nan, device='cuda').half()
+    xd[:M * K], gd[:M * N] = x.cuda().reshape(-1), gy.cuda().reshape(-1)
+    dw = fp8.linear_backward(gd[:M * N].view(M, N), xd[:M * K].view(M, K), None, need_dx=False)[1]
+    want, tol = product_bound(blocks64(gy.t().contiguous(), 'e4m3')[0], blocks64(x.t().contiguous(), 'e4m3')[0], M, torch.float32)
+    check(dw, want, tol)
+
+
+def test_weight_gradient_pitches_and_types(fp8):
+    r = torch.Generator().manual_seed(0)
+    base_x, base_g = torch.randn(500, 301, generator=r).half(), torch.randn(500, 205, generator=r).half()
+    for xs, gs in ((slice(5, 140), slice(3, 80)), (slice(0, 301), slice(204, 205)), (slice(1, 257), slice(0, 128))):
+        x, gy = base_x[:, xs], base_g[:, gs]
+        want, tol = product_bound(blocks64(gy.t().contiguous(), 'e5m2')[0], blocks64(x.t().contiguous(), 'e4m3')[0], 500, torch.float32)
+        check(fp8.linear_backward(base_g.cuda()[:, gs], base_x.cuda()[:, xs], None, 'e5m2', need_dx=False)[1], want, tol)
+        # g and x of different types: 16-bit beside fp32
+        check(fp8.linear_backward(base_g.cuda()[:, gs].float(), base_x.cuda()[:, xs], None, 'e5m2', need_dx=False)[1], want, tol)
+
+
+def test_weight_gradient_nonfinite_columns_stay_in_their_columns(fp8):
+    r = torch.Generator().manual_seed(0)
+    x, gy = torch.randn(1000, 70, generator=r).half(), torch.randn(1000, 40, generator=r).half()
+    x[300, 11], x[999, 69], gy[0, 3], gy[500, 39] = math.inf, math.nan, -math.inf, math.nan
+    for fmt in ('e4m3', 'e5m2'):
+        dw = fp8.linear_backward(gy.cuda(), x.cuda(), None, fmt, need_dx=False)[1].cpu()
+        bad = torch.zeros(40, 70, dtype=torch.bool)
+        bad[:, [11, 69]] = True
+        bad[[3, 39]] = True
+        assert torch.isnan(dw[bad]).all() and torch.isfinite(dw[~bad]).all()
 
 
 def test_linear_nonfinite_rows_stay_in_their_rows(fp8):
