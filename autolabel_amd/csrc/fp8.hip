@@ -224,8 +224,9 @@ __global__ __launch_bounds__(256) void k_fp8_quant_t(const void* __restrict__ x,
 }
 
 // -------------------------------------------------------------------------------------------------------------- products
-template <int FA, int FB> __device__ inline f32x16 mfma8(i32x8 a, i32x8 b, f32x16 c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, 0, sa, 0, sb);
+// SA, SB: which byte of the words of scales
+template <int FA, int FB, int SA = 0, int SB = 0> __device__ inline f32x16 mfma8(i32x8 a, i32x8 b, f32x16 c, int sa, int sb) {
+  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, SA, sa, SB, sb);
 }
 
 // two 8-bit values (the upper two of the word with HI) times a power of two, exact in bf16
@@ -427,16 +428,13 @@ struct Fp8Linear {
 };
 template <int NKB> constexpr int lin_threads() { return NKB <= 4 ? 1024 : 512; }
 
-template <int FA, int FB, int SA, int SB> __device__ inline f32x16 mfma8s(i32x8 a, i32x8 b, f32x16 c, int sa, int sb) {
-  return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, SA, sa, SB, sb);
-}
 template <int FX, int NKB, int KB = 0> __device__ inline void lin_chain(f32x16& acc, const i32x8 (&w)[NKB][2], const uint32_t* sw, const uint32_t* sx, const uint8_t* x, const int (&off)[4]) {
   if constexpr (KB < NKB) {
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       const uint8_t* t = x + KB * 64 * 128;
       const i32x8 f = __builtin_shufflevector(*(const i32x4*)(t + off[2 * ks]), *(const i32x4*)(t + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
-      acc = mfma8s<F8_E4M3, FX, KB & 3, KB & 3>(w[KB][ks], f, acc, (int)sw[KB / 4], (int)sx[KB / 4]);
+      acc = mfma8<F8_E4M3, FX, KB & 3, KB & 3>(w[KB][ks], f, acc, (int)sw[KB / 4], (int)sx[KB / 4]);
     }
     lin_chain<FX, NKB, KB + 1>(acc, w, sw, sx, x, off);
   }
@@ -700,8 +698,6 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
     if (FG != F8_E4M3 && strip < TN / 32) tn_quant<T, FG>(v, t, sc, lane);
     else tn_quant<T, F8_E4M3>(v, t, sc, lane);
   };
-  // Waves 4 .. 7 sit on the same SIMDs as 0 .. 3: with a lower priority they fall behind, and one of a pair multiplies while the other cuts.
-  if (wave < 4) __builtin_amdgcn_s_setprio(1);
   const bool busy = n0 + wn * 32 * NI < p.N && k0 + wk * 64 < p.K;      // (waves without results only cut)
   load(s0, wave);
   const int64_t halves = 2 * (s1 - s0 + 1);
