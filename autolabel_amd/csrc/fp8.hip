@@ -151,7 +151,8 @@ template <int T, int FMT> __device__ inline uint2 quant8(const Eight<T>& x, cons
 }
 
 // ------------------------------------------------------------------------------------------------------------ quantisers
-// Rows: 16 lanes hold a block (8 values each), its maximum goes round them with four DPP steps; one read of x, one write of q.
+// Rows: 16 lanes hold a block (8 values each), its maximum goes round them with four DPP steps; one read of x, one write of q.  Bound by memory:
+// 8192 x 4096 fp16 17.7 us (5.7 TB/s, its input in the memory-side cache), 262144 x 512 79 us (5.1 TB/s; a large copy reaches 4.6).
 template <int T, int FMT>
 __global__ __launch_bounds__(256) void k_fp8_quant(const void* __restrict__ x, int64_t ldx, int64_t M, int K, int nb, uint8_t* __restrict__ q,
                                                    int64_t ldq, uint8_t* __restrict__ scale, int64_t lds) {
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(256) void k_fp8_quant(const void* __restrict__ x, i
 
 // Columns: q of x^T with blocks of 128 along the rows of x.  A block of threads turns a tile of 128 rows x 64 columns round: a thread reads
 // eight columns of four rows, the maxima of a column meet through three shuffles and LDS, the 8-bit values cross in LDS and leave as whole
-// 128-byte lines.
+// 128-byte lines.  262144 x 512 fp16 101 us, 4.0 TB/s: the two barriers of a tile, with nothing of the next one in flight, are what is left.
 template <int T, int FMT>
 __global__ __launch_bounds__(256) void k_fp8_quant_t(const void* __restrict__ x, int64_t ldx, int64_t M, int C, int nb, uint8_t* __restrict__ q,
                                                      int64_t ldq, uint8_t* __restrict__ scale, int64_t lds) {
@@ -292,6 +293,16 @@ __device__ inline void store_block(const Fp8Out& o, const f32x16& c0, const f32x
   __builtin_amdgcn_wave_barrier();
 }
 
+// Blocks b and b + 8 run on the same XCD.  Each XCD takes a run of consecutive work items, so that those that share rows find them in its L2, and
+// all eight have the same number, however few there are: with the row tiles going round the XCDs instead, the one row tile of 64 x 4096 x 4096 was
+// work for 32 of the 256 CUs (40.6 us, so 15.0), and 128 parts of 64 x 512 x 4096 too (18.7, so 5.6).  -1: none left for this block of a grid of
+// xcd_grid(items).
+__device__ inline int xcd_item(int items) {
+  const int each = (items + 7) / 8, i = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+  return i < items ? i : -1;
+}
+static inline uint32_t xcd_grid(int64_t items) { return (uint32_t)((items + 7) / 8 * 8); }
+
 // The slot of piece c of row r in a tile of 128-byte rows is c ^ turn(r)
 __device__ inline int turn(int row) { return (row >> 1) & 7; }
 
@@ -303,21 +314,28 @@ struct Fp8NT {
   Fp8Out o;
 };
 
-// y = A B^T.  A tile of 128-byte rows lies in LDS with its 16-byte pieces turned by the row number (piece c of row r in slot c ^ (r & 7)), on
-// both sides of the direct global -> LDS copy: reads of 32 rows then meet every bank evenly.  Which bytes of a 128-block meet in which lane of
-// the matrix instruction is free (both operands use the same order and the block has one scale), so a lane takes pieces 4 h .. 4 h + 3.
+// y = A B^T.  A tile of 128-byte rows lies in LDS with its 16-byte pieces turned by the row number (turn), on both sides of the direct
+// global -> LDS copy: reads of 32 rows then meet every bank evenly (4% of the reads' cycles are conflicts).  Which bytes of a 128-block meet in
+// which lane of the matrix instruction is free (both operands use the same order and the block has one scale), so a lane takes pieces 4 h .. 4 h + 3.
+// Two buffers, one barrier per 128 columns: the next step's copies are sent before this one is multiplied.
 // WIDE: the fp32 results' form, 16-bit operands out of the same tiles.
+// Tiles: 256 x 256 by eight waves, or 128 x 128 by four (nt_type), and the contraction in parts where there are few (nt_plan).
+// 8192 x 4096 x 4096 with 16-bit results: 125 .. 134 us by the card's temperature, 2.05 .. 2.2 PFLOP/s (the library's product of unscaled 8-bit
+// values 112); fp32 results 242 us; 256 x 512 x 4096 13 us with the joining of its parts.
+// What bounds the large ones, in clocks of a CU per 256 x 256 x 128 step: 2050 for the 32 matrix instructions of a SIMD, 170 for the scales, 490 for
+// waves that wait for each other at the barrier, 450 .. 1000 for the 64 KB copied.  Reading the fragments of a half step ahead across the barrier,
+// copies spread between the matrix instructions (through buffer descriptors, without a branch in the loop), 128 x 128 results a wave with one wave per
+// SIMD, and 4 x 8 groups of tiles per XCD were built and took 144 .. 178 us where this takes 145.
 template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI>
 __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
   constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, ROWS = BM + BN;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem8[];    // [2][ROWS][128]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
   const int wm = wave % WM, wn = wave / WM;
-  // blocks b and b + 8 run on the same XCD: the column tiles of a row tile go there back to back and find its rows in that L2
-  const int ntn = (p.N + BN - 1) / BN, xcd = blockIdx.x & 7, jj = blockIdx.x >> 3;
-  const int64_t m0 = ((int64_t)(jj / ntn) * 8 + xcd) * BM;
-  const int n0 = (jj % ntn) * BN;
-  if (m0 >= p.M) return;
+  const int ntn = (p.N + BN - 1) / BN, tile = xcd_item((int)((p.M + BM - 1) / BM) * ntn);      // the column tiles of a row tile follow each other
+  if (tile < 0) return;
+  const int64_t m0 = (int64_t)(tile / ntn) * BM;
+  const int n0 = (tile % ntn) * BN;
   const int kb0 = blockIdx.y * p.per, kb1 = min(p.nkb, kb0 + p.per);
   f32x16 acc[NI][MI];
 #pragma unroll
@@ -418,12 +436,16 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
 // range of rows and goes through it in tiles of up to 64: a tile's rows are cut into 8-bit blocks in one LDS buffer (four lanes to a block, its
 // power of two worked out once for 32 values) while the tile before it is multiplied out of the other and the loads of the one after it are in
 // flight.  One barrier per tile.
+// Bound by memory where there are many rows: 2^20 x 512 x 512 fp16 479 us, 4.5 TB/s (a large copy reaches 4.6).  50000 rows are four tiles to a block
+// and take 34 us (3.0 TB/s): the first tile's loads and the last one's results have nothing beside them, and tiles of 32 .. 48 rows instead of 64
+// cost more than they hide (36 .. 37.5 us; 2^20 rows 561 .. 634).  4096 rows 10 us, one row 5 us (a launch, and 256 KB of weights).
+// At NKB 4, 7 and 8 the registers do not quite hold everything: 12 .. 84 bytes a lane lie in scratch and are read once per tile.
 struct Fp8Linear {
   const void* x; int64_t ldx;
   const uint8_t* w; int64_t ldw; const uint8_t* sw; int64_t ldsw;
   int64_t M; int N, K;
   int wn, parts;                  // waves side by side along the columns of y (a power of two); blocks of threads side by side
-  int rows, bm;                   // rows of a block of threads, of a tile (<= 64)
+  int ranges, rows, bm;           // ranges of rows; rows of a range, of a tile (<= 64)
   Fp8Out o;
 };
 template <int NKB> constexpr int lin_threads() { return NKB <= 4 ? 1024 : 512; }
@@ -446,10 +468,9 @@ __global__ __launch_bounds__(lin_threads<NKB>()) void k_fp8_linear(Fp8Linear p) 
   __shared__ __attribute__((aligned(16))) uint8_t xs[2][NKB][64][128];         // 16-byte pieces turned by the row
   __shared__ __attribute__((aligned(16))) uint8_t se[2][64][4 * WORDS];        // exponents + 127
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
-  // blocks b and b + 8 run on the same XCD: the parts of a row range go there and share its rows in that L2
-  const int xcd = blockIdx.x & 7, jj = blockIdx.x >> 3, part = jj % p.parts;
-  const int64_t lo = ((int64_t)(jj / p.parts) * 8 + xcd) * p.rows, hi = lo + p.rows < p.M ? lo + p.rows : p.M;
-  if (lo >= hi) return;
+  const int item = xcd_item(p.ranges * p.parts), part = item % p.parts;       // the parts of a row range follow each other
+  if (item < 0) return;
+  const int64_t lo = (int64_t)(item / p.parts) * p.rows, hi = lo + p.rows < p.M ? lo + p.rows : p.M;
   const int wn = wave % p.wn, wm = wave / p.wn, step = NW / p.wn, n0 = (part * p.wn + wn) * 32;
   Eight<T> v[ROUNDS][4];
   // (a uniform base and a 32-bit offset of the lane in bytes: pitches are under 2^25.  Rows behind the tile's last are read as that one: what is
@@ -565,10 +586,14 @@ __global__ __launch_bounds__(lin_threads<NKB>()) void k_fp8_linear(Fp8Linear p) 
 // load instruction reads 64 bytes of 16 rows), pairs up its rows (v_perm), the column's maximum crosses the 16 lanes of a DPP row, and each
 // column leaves as 128 bytes of 8-bit values.  Both operands carry the same order of the rows, whatever it is.
 // Two LDS buffers: while a step is multiplied the strips of the next one are cut into blocks, and the loads of the strip after that are in flight.
+// 2^19 x 512 x 512 fp16: 393 us (0.70 PFLOP/s, and 1.07 GB at 2.7 TB/s).  Every value is read by two blocks (of the same XCD) and cut by both; the
+// matrix instructions of a SIMD take 35% of the time, the vector ones that cut and widen most of the rest, and this pattern of loads alone 300 us.
+// Strips of 64 columns by pairs of waves (128-byte pieces of 8 rows, 214 us alone) need a third barrier and took 417 us, two strips on their way per
+// wave 395, sixteen waves or half strips in turn more registers than there are.
 struct Fp8TN {
   const void* g; int64_t ldg; const void* x; int64_t ldx;
   int64_t M; int N, K;
-  int tn, tk, per;                // tiles of the result, steps of a part
+  int tn, tk, parts, per;         // tiles of the result, parts of the rows, steps of a part
   float* y;                       // [parts][N][K]
 };
 
@@ -623,8 +648,8 @@ template <int T, int FMT> __device__ inline void tn_quant(u16x8 (&v)[8], uint8_t
   if (rg == 0) { *(f32x4*)(scale + c8) = (f32x4){s[0], s[1], s[2], s[3]}; *(f32x4*)(scale + c8 + 4) = (f32x4){s[4], s[5], s[6], s[7]}; }
 }
 
-// TAIL: the last step is not whole or its pieces would reach over the tensors' end; the code for that costs the others registers (630 us -> 660
-// at 2^19 rows x 512 x 512, where there is none).
+// TAIL: the last step is not whole or its pieces would reach over the tensors' end; the code for that costs the others registers (with dx, 630 us
+// -> 660 at 2^19 x 512 x 512, where there is none).
 template <int T, int FG, int NI, bool TAIL>
 __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
   constexpr int TN = 64 * NI, TK = 256, COLS = TN + TK, STRIPS = COLS / 32;      // 8 < STRIPS <= 16
@@ -632,10 +657,9 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
   float* scales = (float*)(smem8 + 2 * COLS * 128);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5;
   const int wn = wave & 1, wk = wave >> 1;                // waves: 2 along n (32 NI columns each), 4 along k (64 each)
-  // blocks b and b + 8 run on the same XCD: the tiles of a part go there back to back and share its rows in that L2
-  const int tiles = p.tn * p.tk, xcd = blockIdx.x & 7, jj = blockIdx.x >> 3, part = (jj / tiles) * 8 + xcd, tile = jj % tiles;
+  const int tiles = p.tn * p.tk, item = xcd_item(p.parts * tiles), part = item / tiles, tile = item % tiles;     // the tiles of a part follow each other
+  if (item < 0) return;
   const int64_t nsteps = (p.M + 127) / 128, s0 = (int64_t)part * p.per, s1 = s0 + p.per < nsteps ? s0 + p.per : nsteps;
-  if (s0 >= nsteps) return;
   const int n0 = tile / p.tk * TN, k0 = tile % p.tk * TK;
   f32x16 acc[NI][2];
 #pragma unroll
@@ -761,7 +785,7 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
 }
 
 // The slabs of a split contraction, added in a fixed order and rounded once.  Eight threads share four results (their slabs' sums meet through
-// shuffles): with a result's slabs read by one thread alone, 85 slabs of 128 x 512 took 22 us.
+// shuffles): with a result's slabs read by one thread alone, 85 slabs of 128 x 512 took 22 us, so 6.8; 64 slabs of 512 x 512 take 15 us, 4.5 TB/s.
 __global__ __launch_bounds__(256) void k_fp8_join(const float* __restrict__ slabs, int splits, int64_t M, int N, Fp8Out o) {
   const int64_t n = M * N;
   for (int64_t q = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3; q < (n + 3) / 4; q += (int64_t)gridDim.x * 32) {
@@ -836,15 +860,21 @@ extern "C" int aln_fp8_quantize_t(const void* x, int32_t x_type, int64_t ldx, in
   return quantize("fp8_quantize_t", true, x, x_type, ldx, M, C, fmt, q, ldq, scale, lds, (hipStream_t)stream);
 }
 
-// How a product is cut: tiles of y, and parts of the contraction where the tiles alone leave most of the 256 CUs without work.
+// How a product is cut: tiles of y, and parts of the contraction where the tiles alone leave CUs without work.  A step of 128 x 128 x 128 takes a
+// lone block on its CU about 0.8 us; joining the parts costs a launch (4 us) and their slabs' way through the memory-side cache and back.  With
+// and without parts: 256 x 512 x 4096 12.7 us and 24.2, 64 x 1024 x 4096 11.0 and 28.2, 1024 x 1024 x 4096 22.6 and 29.8; but 1920 x 1024 x 2048 in
+// four parts 26.4 and 15.6 in one.
 struct NtPlan { int splits, per; };
 static NtPlan nt_plan(int64_t M, int N, int64_t K) {
   const int64_t tiles = (M + 127) / 128 * ((N + 127) / 128), nkb = ceil128(K) / 128;
-  int64_t s = tiles >= 256 ? 1 : 512 / tiles;
-  if (s > nkb / 4) s = nkb / 4;
-  if (s < 1) s = 1;
-  const int64_t per = ((nkb + s - 1) / s + 3) / 4 * 4;    // (whole words of scales)
-  return {(int)((nkb + per - 1) / per), (int)per};
+  NtPlan best{1, (int)((nkb + 3) / 4 * 4)};
+  double least = 0.8 * nkb;
+  for (int64_t s = 2; s * tiles <= 256 && 4 * s <= nkb; ++s) {
+    const int64_t per = ((nkb + s - 1) / s + 3) / 4 * 4, parts = (nkb + per - 1) / per;    // (whole words of scales)
+    const double t = 0.8 * per + 4.0 + 2e-6 * parts * M * N;
+    if (t < least) { least = t; best = {(int)parts, (int)per}; }
+  }
+  return best;
 }
 extern "C" int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K) {
   if (M <= 0 || N <= 0 || K <= 0) return 0;
@@ -855,14 +885,17 @@ template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI> static int 
   constexpr int BM = WM * MI * 32, BN = WN * NI * 32, LDS = 2 * (BM + BN) * 128;
   static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_nt: %s", hipGetErrorString(big));
-  const int64_t g = ((p.M + BM - 1) / BM + 7) / 8 * 8 * ((p.N + BN - 1) / BN);
+  const int64_t g = (p.M + BM - 1) / BM * ((p.N + BN - 1) / BN);
   ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_nt: %lld x %d results are too many for one launch", (long long)p.M, p.N);
-  hipLaunchKernelGGL((k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>), dim3((uint32_t)g, p.splits), dim3(64 * WM * WN), LDS, st, p);
+  hipLaunchKernelGGL((k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>), dim3(xcd_grid(g), p.splits), dim3(64 * WM * WN), LDS, st, p);
   ALN_CHECK_LAUNCH("fp8_nt");
   return 0;
 }
 template <int FA, int FB> static int nt_type(const Fp8NT& p, int y_type, hipStream_t st) {
-  const bool big = (p.M + 255) / 256 * ((p.N + 255) / 256) >= 256;
+  // rounds of the 256 CUs: one 256 x 256 tile at a time takes 4 / 3 of the time of two 128 x 128 ones.  Large and small tiles: 4096 x 4096 x 4096 65.5 us and
+  // 88.5, 3840 x 3840 x 2048 33.6 and 44.7, 8192 x 4096 x 1024 40.6 and 52.4, but 2048 x 4096 x 4096 57.0 and 43.7
+  const int64_t large = (p.M + 255) / 256 * ((p.N + 255) / 256), small = (p.M + 127) / 128 * ((p.N + 127) / 128);
+  const bool big = 4 * ((large + 255) / 256) <= 3 * ((small + 511) / 512);
   if (y_type == FT_F32) return big ? nt_launch<FA, FB, true, 2, 4, 4, 2>(p, st) : nt_launch<FA, FB, true, 2, 2, 2, 2>(p, st);
   return big ? nt_launch<FA, FB, false, 2, 4, 4, 2>(p, st) : nt_launch<FA, FB, false, 2, 2, 2, 2>(p, st);
 }
@@ -890,23 +923,24 @@ extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t
   return 0;
 }
 
-// ---- x W^T for x as it is.  16-bit x and y, e4m3 weights, up to 512 columns (1024 with few columns of y): the one-launch kernel; otherwise blocks of
-// x in the workspace, then the product.
-// (eight waves hold 256 columns of y at 513 .. 1024 columns of x, and every further part cuts the rows again: 4096 x 768 x 768 takes 12.8 us, 14.9 in
-// two launches, but 8192 x 1024 x 1024 27.2, 25.3 in two, and 8192 x 1024 x 4096 65.8, 49.5 in two; up to 512 columns 131072 x 512 x 4096 482, 557 in two)
-static bool lin_fused(int N, int64_t K, int x_type, int y_type, int fmt_w) {
-  return (K <= 512 || (K <= 1024 && N <= 768)) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
+// ---- x W^T for x as it is.  16-bit x and y, e4m3 weights, up to 512 columns (1024 with few rows or few columns of y): the one-launch kernel;
+// otherwise blocks of x in the workspace, then the product.
+// (eight waves hold 256 columns of y at 513 .. 1024 columns of x, and every further part cuts the rows again.  In one launch and in two: 64 x 1024 x 4096
+// 8.9 us and 14.0, 1024 x 1024 x 4096 16.9 and 16.6, 8192 x 1024 x 4096 62 and 50, 8192 x 640 x 4096 44 and 38, 8192 x 1024 x 1024 24 either way, 65537 x 1024
+// x 512 80 and 95; up to 512 columns 131072 x 512 x 4096 482 and 557)
+static bool lin_fused(int64_t M, int N, int64_t K, int x_type, int y_type, int fmt_w) {
+  return (K <= 512 || (K <= 1024 && (N <= 1024 || M <= 512))) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
 }
 static inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t x_type, int32_t y_type, int32_t fmt_w) {
-  if (M <= 0 || N <= 0 || K <= 0 || lin_fused(N, K, x_type, y_type, fmt_w)) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || lin_fused(M, N, K, x_type, y_type, fmt_w)) return 0;
   const int64_t nb = ceil128(K) / 128;
   return M * nb * 128 + up16(M * ((nb + 3) / 4 * 4)) + aln_fp8_nt_ws_bytes(M, N, K);
 }
 template <int T, int FX, int NKB> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
-  const int64_t g = ((p.M + p.rows - 1) / p.rows + 7) / 8 * 8 * p.parts;
+  const int64_t g = (int64_t)p.ranges * p.parts;
   ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_linear: %lld x %d results are too many for one launch", (long long)p.M, p.N);
-  hipLaunchKernelGGL((k_fp8_linear<T, FX, NKB>), dim3((uint32_t)g), dim3(lin_threads<NKB>()), 0, st, p);
+  hipLaunchKernelGGL((k_fp8_linear<T, FX, NKB>), dim3(xcd_grid(g)), dim3(lin_threads<NKB>()), 0, st, p);
   ALN_CHECK_LAUNCH("fp8_linear");
   return 0;
 }
@@ -933,14 +967,15 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
   const int64_t need = aln_fp8_linear_ws_bytes(M, N, K, x_type, y_type, fmt_w);
   ALN_REQUIRE(ws_bytes >= need && (need == 0 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_linear: the workspace needs %lld bytes, aligned to 16", (long long)need);
   const int nkb = (int)(ceil128(K) / 128);
-  if (!lin_fused(N, K, x_type, y_type, fmt_w)) {
+  if (!lin_fused(M, N, K, x_type, y_type, fmt_w)) {
     uint8_t* q = (uint8_t*)ws, *sc = q + M * nkb * 128, *rest = sc + up16(M * ((nkb + 3) / 4 * 4));
     const int rc = aln_fp8_quantize(x, x_type, ldx, M, K, fmt_x, q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, stream);
     if (rc) return rc;
     return aln_fp8_nt(q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, fmt_x, w, ldw, sw, ldsw, fmt_w, M, N, K, y, ldy, y_type, relu, rest, ws_bytes - (rest - q), stream);
   }
   // One block of threads per CU.  While there are fewer 64-row tiles than CUs the columns of y are cut into more parts (each cuts the rows
-  // into blocks again); the rows then go round evenly, in tiles of one size.
+  // into blocks again); the rows then go round evenly, in tiles of one size.  512 x 512 weights with these parts and with one part: 64 rows 5.4 us and
+  // 12.3, 4096 rows 10.0 and 13.5, 8192 rows 14.3 and 14.9, the same from 16384 rows on.
   const int waves = nkb <= 4 ? 16 : 8, need_wn = (N + 31) / 32;
   const int64_t mt = (M + 63) / 64;
   int wn = 1;
@@ -950,7 +985,7 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
   if (blocks > mt) blocks = mt;
   const int64_t rows = (M + blocks - 1) / blocks, tiles = (rows + 63) / 64;
   ALN_REQUIRE(rows < (int64_t)1 << 31, "fp8_linear: too many rows");
-  const Fp8Linear p{x, ldx, (const uint8_t*)w, ldw, sw, ldsw, M, N, K, wn, parts, (int)rows, (int)((rows + tiles - 1) / tiles), Fp8Out{y, ldy, y_type, relu}};
+  const Fp8Linear p{x, ldx, (const uint8_t*)w, ldw, sw, ldsw, M, N, K, wn, parts, (int)((M + rows - 1) / rows), (int)rows, (int)((rows + tiles - 1) / tiles), Fp8Out{y, ldy, y_type, relu}};
   hipStream_t st = (hipStream_t)stream;
   return x_type == FT_F16 ? (fmt_x == F8_E4M3 ? lin_pick<FT_F16, F8_E4M3>(p, nkb, st) : lin_pick<FT_F16, F8_E5M2>(p, nkb, st))
                           : (fmt_x == F8_E4M3 ? lin_pick<FT_BF16, F8_E4M3>(p, nkb, st) : lin_pick<FT_BF16, F8_E5M2>(p, nkb, st));
@@ -962,12 +997,13 @@ static bool tn_fused(int64_t M, int N, int K, int g_type, int x_type) { return g
 struct TnPlan { int ni, tn, tk, parts, per; };
 static TnPlan tn_plan(int64_t M, int N, int K) {
   TnPlan t;
-  // 256 x 256 results to a block cut every value of g and x half as often as 128 x 256 do, where there are blocks enough for every CU
+  // 256 x 256 results to a block cut every value of g and x half as often as 128 x 256 do, where there are blocks enough for every CU: 2^19 x 512 x 512
+  // 470 us against 609, 16384 x 1024 x 1024 75 against 84, but 8192 x 512 x 512 32.1 against 27.6 and 4096 x 512 x 512 29.1 against 24.2
   t.ni = N > 128 && (N + 255) / 256 * (int64_t)((K + 255) / 256) * ((M + 127) / 128) >= 512 ? 4 : 2;
   t.tn = (N + 64 * t.ni - 1) / (64 * t.ni); t.tk = (K + 255) / 256;
   const int64_t tiles = (int64_t)t.tn * t.tk, steps = (M + 127) / 128;
   int64_t parts = tiles >= 256 ? 1 : 256 / tiles;         // one block per CU
-  // two steps at least, where the parts' slabs are more than small change
+  // two steps at least, where the parts' slabs are more than small change (4096 x 512 x 512 24.2 us, 25.9 with one step to a part)
   if (parts * N * K > 1 << 20 && parts > (steps + 1) / 2) parts = (steps + 1) / 2;
   if (parts > steps) parts = steps;
   t.per = (int)((steps + parts - 1) / parts);
@@ -980,22 +1016,22 @@ extern "C" int64_t aln_fp8_grad_weight_ws_bytes(int64_t M, int32_t N, int32_t K,
   const int64_t nb = ceil128(M) / 128, per_row = nb * 128 + (nb + 3) / 4 * 4;
   return up16(((int64_t)N + K) * per_row) + 16 * 4 + aln_fp8_nt_ws_bytes(N, K, M);
 }
-template <int T, int FG, int NI, bool TAIL> static int tn_launch(const Fp8TN& p, int parts, hipStream_t st) {
+template <int T, int FG, int NI, bool TAIL> static int tn_launch(const Fp8TN& p, hipStream_t st) {
   constexpr int COLS = 64 * NI + 256, LDS = 2 * COLS * 132;
   static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI, TAIL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_grad_weight: %s", hipGetErrorString(big));
-  const int64_t g = (int64_t)(parts + 7) / 8 * 8 * p.tn * p.tk;
+  const int64_t g = (int64_t)p.parts * p.tn * p.tk;
   ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_grad_weight: %d x %d results are too many for one launch", p.N, p.K);
-  hipLaunchKernelGGL((k_fp8_tn<T, FG, NI, TAIL>), dim3((uint32_t)g), dim3(512), LDS, st, p);
+  hipLaunchKernelGGL((k_fp8_tn<T, FG, NI, TAIL>), dim3(xcd_grid(g)), dim3(512), LDS, st, p);
   ALN_CHECK_LAUNCH("fp8_grad_weight");
   return 0;
 }
-template <int T, int FG, int NI> static int tn_tail(const Fp8TN& p, int parts, hipStream_t st) {
-  return p.M % 128 || p.N % 32 || p.K % 32 ? tn_launch<T, FG, NI, true>(p, parts, st) : tn_launch<T, FG, NI, false>(p, parts, st);
+template <int T, int FG, int NI> static int tn_tail(const Fp8TN& p, hipStream_t st) {
+  return p.M % 128 || p.N % 32 || p.K % 32 ? tn_launch<T, FG, NI, true>(p, st) : tn_launch<T, FG, NI, false>(p, st);
 }
 template <int T> static int tn_pick(const Fp8TN& p, const TnPlan& t, int fmt_g, hipStream_t st) {
-  if (fmt_g == F8_E4M3) return t.ni == 4 ? tn_tail<T, F8_E4M3, 4>(p, t.parts, st) : tn_tail<T, F8_E4M3, 2>(p, t.parts, st);
-  return t.ni == 4 ? tn_tail<T, F8_E5M2, 4>(p, t.parts, st) : tn_tail<T, F8_E5M2, 2>(p, t.parts, st);
+  if (fmt_g == F8_E4M3) return t.ni == 4 ? tn_tail<T, F8_E4M3, 4>(p, st) : tn_tail<T, F8_E4M3, 2>(p, st);
+  return t.ni == 4 ? tn_tail<T, F8_E5M2, 4>(p, st) : tn_tail<T, F8_E5M2, 2>(p, st);
 }
 extern "C" int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, int32_t fmt_g, const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t N, int32_t K,
                                    float* dw, void* ws, int64_t ws_bytes, void* stream) {
@@ -1016,7 +1052,7 @@ extern "C" int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, i
     return aln_fp8_nt(qg, ld, sg, lds, fmt_g, qx, ld, sx, lds, F8_E4M3, N, K, M, dw, K, FT_F32, 0, rest, ws_bytes - (rest - qg), stream);
   }
   const TnPlan t = tn_plan(M, N, K);
-  const Fp8TN p{g, ldg, x, ldx, M, N, K, t.tn, t.tk, t.per, t.parts > 1 ? (float*)ws : dw};
+  const Fp8TN p{g, ldg, x, ldx, M, N, K, t.tn, t.tk, t.parts, t.per, t.parts > 1 ? (float*)ws : dw};
   const int rc = g_type == FT_F16 ? tn_pick<FT_F16>(p, t, fmt_g, st) : tn_pick<FT_BF16>(p, t, fmt_g, st);
   if (rc || t.parts == 1) return rc;
   hipLaunchKernelGGL(k_fp8_join, dim3(aln_grid_for(((int64_t)N * K + 3) / 4, 32, 4096)), dim3(256), 0, st, (const float*)ws, t.parts, (int64_t)N, K, Fp8Out{dw, K, FT_F32, 0});
