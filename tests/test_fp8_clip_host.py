@@ -155,3 +155,43 @@ def test_autoencoder_keeps_its_parameters():
     assert all(torch.equal(x, y) for x, y in zip(a.state_dict().values(), b.state_dict().values()))
     with pytest.raises(ValueError, match='no CPU path'):
         b(torch.zeros(2, 32))
+
+
+LINEAR = dict(x=A, x_type=0, ldx=200, fmt_x=0, w=A, ldw=256, sw=A, ldsw=4, fmt_w=0, M=4, N=8, K=200, y=A, ldy=8, y_type=0, relu=0, ws=None, ws_bytes=0, stream=None)
+GRAD = dict(g=A, g_type=0, ldg=8, fmt_g=1, x=A, x_type=0, ldx=200, M=1000, N=8, K=200, dw=A, ws=A, ws_bytes=1 << 30, stream=None)
+
+
+@pytest.mark.parametrize('bad, match', [
+    (dict(x_type=3), 'unknown type'), (dict(y_type=-1), 'unknown type'), (dict(fmt_x=2), 'unknown type'), (dict(fmt_w=-1), 'unknown type'), (dict(M=-1), 'sizes'),
+    (dict(M=1 << 31), 'sizes'), (dict(N=0), 'sizes'), (dict(K=0), 'sizes'), (dict(ldy=7), 'sizes'), (dict(ldx=-1), 'sizes'), (dict(ldx=1 << 25), 'sizes'), (dict(ldy=1 << 25), 'sizes'),
+    (dict(w=None), '8-bit blocks'), (dict(w=A + 8), '8-bit blocks'), (dict(ldw=128), '8-bit blocks'), (dict(sw=None), '8-bit blocks'), (dict(ldsw=2), '8-bit blocks'),
+    (dict(x=None), 'x or y is NULL'), (dict(y=None), 'x or y is NULL'), (dict(x=A + 1), 'not aligned'), (dict(y=A + 2, y_type=2), 'not aligned'),
+    (dict(x_type=2), 'workspace'), (dict(x_type=2, ws=A + 8, ws_bytes=1 << 30), 'workspace'), (dict(fmt_w=1, ws=A, ws_bytes=100), 'workspace'),
+])
+def test_linear_c_refusals(bad, match):
+    with pytest.raises(RuntimeError, match=match):
+        hip.call('aln_fp8_linear', *{**LINEAR, **bad}.values())
+
+
+@pytest.mark.parametrize('bad, match', [
+    (dict(g_type=3), 'unknown type'), (dict(x_type=-1), 'unknown type'), (dict(fmt_g=2), 'unknown type'), (dict(M=0), 'sizes'), (dict(M=1 << 31), 'sizes'), (dict(N=0), 'sizes'),
+    (dict(K=0), 'sizes'), (dict(ldg=7), 'sizes'), (dict(ldx=199), 'sizes'), (dict(ldg=1 << 24), 'sizes'), (dict(ldx=1 << 24), 'sizes'), (dict(g=None), 'NULL'), (dict(x=None), 'NULL'),
+    (dict(dw=None), 'NULL'), (dict(g=A + 1), 'not aligned'), (dict(dw=A + 2), 'not aligned'), (dict(ws=None), 'workspace'), (dict(ws_bytes=64), 'workspace'), (dict(ws=A + 4), 'workspace'),
+    (dict(g_type=2, ws_bytes=4096), 'workspace'),
+])
+def test_grad_weight_c_refusals(bad, match):
+    with pytest.raises(RuntimeError, match=match):
+        hip.call('aln_fp8_grad_weight', *{**GRAD, **bad}.values())
+
+
+def test_product_workspaces_follow_the_call():
+    """No workspace where one launch does it; with one, room for the blocks of x and for the parts of a split contraction."""
+    L = hip.lib()
+    assert L.aln_fp8_linear_ws_bytes(1 << 20, 4096, 512, 0, 0, 0) == 0 and L.aln_fp8_linear_ws_bytes(1, 4096, 1024, 1, 0, 0) == 0
+    for sizes in ((1 << 20, 4096, 512, 2, 0, 0), (1 << 20, 4096, 512, 0, 2, 0), (1 << 20, 4096, 512, 0, 0, 1), (8192, 4096, 1024, 0, 0, 0), (1, 1, 1025, 0, 0, 0)):
+        m, n, k = sizes[:3]
+        assert L.aln_fp8_linear_ws_bytes(*sizes) >= m * -(-k // 128) * 129 + L.aln_fp8_nt_ws_bytes(m, n, k)
+    for m, n, k in ((1, 1, 1), (1003, 130, 77), (1 << 19, 512, 512), (43200, 128, 512)):
+        assert L.aln_fp8_grad_weight_ws_bytes(m, n, k, 0, 0) % (4 * n * k) == 0
+        assert L.aln_fp8_grad_weight_ws_bytes(m, n, k, 2, 0) >= (n + k) * -(-m // 128) * 129
+    assert L.aln_fp8_grad_weight_ws_bytes(0, 5, 5, 0, 0) == 0 and L.aln_fp8_linear_ws_bytes(0, 5, 5, 2, 0, 0) == 0

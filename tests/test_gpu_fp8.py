@@ -426,3 +426,30 @@ def test_gpu_refusals(fp8):
         fp8.linear_backward(x[:3], x, w)
     with pytest.raises(ValueError, match='weight_t is'):
         fp8.linear_backward(x, x, w)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('M,K,N', [(3841, 200, 3777), (64, 1000, 4096), (1000, 700, 1300), (1920, 2048, 1024), (100, 4100, 120), (1100, 130, 2300)])
+def test_matmul_tiles_and_parts(fp8, M, K, N, dtype):
+    """Large and small tiles, one row tile and many, numbers of tiles that eight does not divide, contractions in one part and in several."""
+    g = torch.Generator().manual_seed(M + K + N)
+    a, b = torch.randn(M, K, generator=g) * torch.rand(M, 1, generator=g), torch.randn(N, K, generator=g) / math.sqrt(K)
+    want, tol = product_bound(blocks64(a, 'e4m3')[0], blocks64(b, 'e4m3')[0], K, dtype)
+    check(fp8.matmul(fp8.quantize(a.cuda()), fp8.quantize(b.cuda()), dtype), want, tol)
+
+
+@pytest.mark.parametrize('M,K,N', [(1, 1000, 4000), (512, 900, 1100), (513, 900, 1100), (600, 1024, 1024), (64, 500, 4100), (2304, 100, 200), (900, 60, 520)])
+def test_linear_parts(fp8, M, K, N):
+    """Either side of where one launch does it, and row ranges and column parts that eight does not divide."""
+    g = torch.Generator().manual_seed(M + K + N)
+    x, w = (torch.randn(M, K, generator=g) * torch.rand(M, 1, generator=g)).half(), torch.randn(N, K, generator=g) / math.sqrt(K)
+    want, tol = product_bound(blocks64(x, 'e4m3')[0], blocks64(w, 'e4m3')[0], K, torch.float16)
+    check(fp8.linear(x.cuda(), fp8.quantize(w.cuda())), want, tol)
+
+
+@pytest.mark.parametrize('M,K,N', [(1200, 1300, 1100), (300, 2100, 600), (128, 600, 4100)])
+def test_weight_gradient_few_parts(fp8, M, K, N):
+    g = torch.Generator().manual_seed(M + K + N)
+    x, gy = torch.randn(M, K, generator=g).half(), (torch.randn(M, N, generator=g) * 0.1).half()
+    want, tol = product_bound(blocks64(gy.t().contiguous(), 'e5m2')[0], blocks64(x.t().contiguous(), 'e4m3')[0], M, torch.float32)
+    check(fp8.linear_backward(gy.cuda(), x.cuda(), None, 'e5m2', need_dx=False)[1], want, tol)
