@@ -883,7 +883,8 @@ extern "C" int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K) {
 }
 template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI> static int nt_launch(const Fp8NT& p, hipStream_t st) {
   constexpr int BM = WM * MI * 32, BN = WN * NI * 32, LDS = 2 * (BM + BN) * 128;
-  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  // (at every call: it holds for the current device)
+  const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_nt<FA, FB, WIDE, WM, WN, MI, NI>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_nt: %s", hipGetErrorString(big));
   const int64_t g = (p.M + BM - 1) / BM * ((p.N + BN - 1) / BN);
   ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_nt: %lld x %d results are too many for one launch", (long long)p.M, p.N);
@@ -1018,7 +1019,7 @@ extern "C" int64_t aln_fp8_grad_weight_ws_bytes(int64_t M, int32_t N, int32_t K,
 }
 template <int T, int FG, int NI, bool TAIL> static int tn_launch(const Fp8TN& p, hipStream_t st) {
   constexpr int COLS = 64 * NI + 256, LDS = 2 * COLS * 132;
-  static const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI, TAIL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+  const hipError_t big = hipFuncSetAttribute((const void*)k_fp8_tn<T, FG, NI, TAIL>, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
   ALN_REQUIRE(big == hipSuccess, "fp8_grad_weight: %s", hipGetErrorString(big));
   const int64_t g = (int64_t)p.parts * p.tn * p.tk;
   ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_grad_weight: %d x %d results are too many for one launch", p.N, p.K);

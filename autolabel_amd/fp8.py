@@ -168,6 +168,8 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
     if out is not None:
         if not torch.is_tensor(out) or out.shape != (*x.shape[:-1], n) or not out.is_contiguous() or out.get_device() != x.get_device() or out_dtype not in (None, out.dtype):
             raise ValueError(f'linear: out must be a contiguous tensor of shape {(*x.shape[:-1], n)} beside x (of out_dtype, where given)')
+        if out.requires_grad and torch.is_grad_enabled():
+            raise ValueError('linear: out must not require a gradient (autograd does not see what is written into it)')
         out_dtype = out.dtype
     if out_dtype is None:
         out_dtype = x.dtype
@@ -184,6 +186,8 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
         H.call('aln_fp8_linear', rows.data_ptr(), x_type, _pitch(rows), FORMATS[fmt][0], weight.q.data_ptr(), ldw, weight.scale.data_ptr(),
                weight.scale.shape[1], fmt_w, m, n, k, y.data_ptr(), n, y_type, 1 if relu else 0, ws.data_ptr() if nbytes else None, nbytes, H.raw_stream())
+    if out is not None and not out.is_inference():
+        torch.autograd.graph.increment_version(out)      # (a backward pass that saved it notices)
     return y
 
 

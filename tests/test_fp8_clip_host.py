@@ -195,3 +195,12 @@ def test_product_workspaces_follow_the_call():
         assert L.aln_fp8_grad_weight_ws_bytes(m, n, k, 0, 0) % (4 * n * k) == 0
         assert L.aln_fp8_grad_weight_ws_bytes(m, n, k, 2, 0) >= (n + k) * -(-m // 128) * 129
     assert L.aln_fp8_grad_weight_ws_bytes(0, 5, 5, 0, 0) == 0 and L.aln_fp8_linear_ws_bytes(0, 5, 5, 2, 0, 0) == 0
+
+
+def test_linear_out_that_autograd_would_miss():
+    w = fp8.Fp8Blocks(torch.zeros(4, 128).to(torch.float8_e4m3fn), torch.full((4, 4), 127, dtype=torch.uint8), 100)
+    x, out = torch.zeros(3, 100), torch.zeros(3, 4, requires_grad=True)
+    with pytest.raises(ValueError, match='must not require a gradient'):
+        fp8.linear(x, w, out=out)
+    with torch.no_grad(), pytest.raises(ValueError, match='no CPU path'):      # (allowed: it gets as far as the device)
+        fp8.linear(x, w, out=out)

@@ -453,3 +453,17 @@ def test_weight_gradient_few_parts(fp8, M, K, N):
     x, gy = torch.randn(M, K, generator=g).half(), (torch.randn(M, N, generator=g) * 0.1).half()
     want, tol = product_bound(blocks64(gy.t().contiguous(), 'e5m2')[0], blocks64(x.t().contiguous(), 'e4m3')[0], M, torch.float32)
     check(fp8.linear_backward(gy.cuda(), x.cuda(), None, 'e5m2', need_dx=False)[1], want, tol)
+
+
+def test_linear_out_tells_autograd(fp8):
+    """A tensor saved for a backward pass and then written into: the backward pass must refuse, as for torch's own operations."""
+    w = fp8.quantize(torch.eye(64, device='cuda'))
+    x, out = torch.ones(5, 64, device='cuda'), torch.ones(5, 64, device='cuda')
+    leaf = torch.ones(5, 64, device='cuda', requires_grad=True)
+    loss = (leaf * out).sum()
+    fp8.linear(x, w, out=out)
+    with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+        loss.backward()
+    with torch.inference_mode():
+        o = torch.empty(5, 64, device='cuda')
+        assert torch.equal(fp8.linear(x, w, out=o), x)
