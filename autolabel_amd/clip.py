@@ -71,7 +71,7 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
     codes = None                 # the tensors' types, where the quick checks already tell
     if set(map(type, every)) <= _PLAIN and all(map(_T.is_contiguous, every)):
         device, types = set(map(_T.get_device, every)), set(map(_dtype, every))
-        same = out is None or list(map(_T.size, out)) == list(map(_T.size, grads))
+        same = out is None or all(map(_T.is_same_size, out, grads))
         if len(device) == 1 and len(types) == 1 and min(device) >= 0 and types <= TYPES.keys() and same:
             codes = array.array('i', (TYPES[types.pop()],)) * n
     if codes is None or loss_scale is not None or found_inf is not None:
