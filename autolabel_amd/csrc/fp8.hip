@@ -1004,9 +1004,10 @@ static TnPlan tn_plan(int64_t M, int N, int K) {
   t.tn = (N + 64 * t.ni - 1) / (64 * t.ni); t.tk = (K + 255) / 256;
   const int64_t tiles = (int64_t)t.tn * t.tk, steps = (M + 127) / 128;
   int64_t parts = tiles >= 256 ? 1 : 256 / tiles;         // one block per CU
-  // two steps at least, where the parts' slabs are more than small change (4096 x 512 x 512 24.2 us, 25.9 with one step to a part)
-  if (parts * N * K > 1 << 20 && parts > (steps + 1) / 2) parts = (steps + 1) / 2;
   if (parts > steps) parts = steps;
+  // two steps at least, where the parts' slabs are more than small change.  With one step to a part and with two: 1003 x 77 x 130 11.9 us and 16.3,
+  // 1000 x 256 x 256 13.6 and 17.9, 600 x 600 x 600 15.3 and 17.0, but 4096 x 256 x 512 21.2 and 19.4, 4096 x 512 x 512 25.9 and 24.2
+  if (parts * N * K > 1 << 21 && parts > (steps + 1) / 2) parts = (steps + 1) / 2;
   t.per = (int)((steps + parts - 1) / parts);
   t.parts = (int)((steps + t.per - 1) / t.per);
   return t;
