@@ -323,7 +323,8 @@ struct Fp8NT {
 // 8192 x 4096 x 4096 with 16-bit results: 125 .. 134 us by the card's temperature, 2.05 .. 2.2 PFLOP/s (the library's product of unscaled 8-bit
 // values 112); fp32 results 242 us; 256 x 512 x 4096 13 us with the joining of its parts.
 // What bounds the large ones, in clocks of a CU per 256 x 256 x 128 step: 2050 for the 32 matrix instructions of a SIMD, 170 for the scales, 490 for
-// waves that wait for each other at the barrier, 450 .. 1000 for the 64 KB copied.  Reading the fragments of a half step ahead across the barrier,
+// waves that wait for each other at the barrier, 450 .. 1000 for the 64 KB copied (with the fragments that is 256 KB through LDS, all that 128 bytes
+// a clock give in 2050).  Reading the fragments of a half step ahead across the barrier,
 // copies spread between the matrix instructions (through buffer descriptors, without a branch in the loop), 128 x 128 results a wave with one wave per
 // SIMD, and 4 x 8 groups of tiles per XCD were built and took 144 .. 178 us where this takes 145.
 template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI>
