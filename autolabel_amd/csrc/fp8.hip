@@ -580,6 +580,138 @@ __global__ __launch_bounds__(lin_threads<NKB>()) void k_fp8_linear(Fp8Linear p) 
   }
 }
 
+// ... and for more columns than registers hold: the tiles of k_fp8_nt (128 x 128, four waves) with the rows of x cut into blocks on the way into LDS.
+// While a step is multiplied the 32 KB of x and 16 KB of W of the next one are on their way to registers (not straight to LDS: the wait for such
+// copies would wait for x as well).  Every column tile cuts the rows again.  444219 x 1203 x 40 bound by memory: 266 .. 283 us, 3.9 TB/s; 1 x 4096 x 4096
+// 13.6 us with the joining of its parts, 16 MB of weights.
+struct Fp8Cut {
+  const void* x; int64_t ldx;
+  const uint8_t* w; int64_t ldw; const uint8_t* sw; int64_t ldsw;
+  int64_t M; int N, K, nkb, splits, per;         // as in Fp8NT
+  Fp8Out o;
+};
+template <int T, int FX>
+__global__ __launch_bounds__(256, 2) void k_fp8_cut(Fp8Cut p) {
+  __shared__ __attribute__((aligned(16))) uint8_t tiles[2][256][128];      // rows of x, rows of W; 16-byte pieces turned by the row
+  __shared__ uint8_t se[2][128];                                           // exponents + 127 of x
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 31, h = lane >> 5, wm = wave & 1, wn = wave >> 1;
+  const int ntn = (p.N + 127) / 128, item = xcd_item((int)((p.M + 127) / 128) * ntn);       // the column tiles of a row tile follow each other
+  if (item < 0) return;
+  const int64_t m0 = (int64_t)(item / ntn) * 128;
+  const int n0 = item % ntn * 128, kb0 = blockIdx.y * p.per, kb1 = min(p.nkb, kb0 + p.per);
+  // rows behind the last are read as that one: what is made of them is never stored
+  const int l = tid & 3, row = tid >> 2, piece = tid & 7, wrow = tid >> 3;                  // rows of x: row + 64 q, of W: wrow + 32 i
+  const uint16_t* px[2];
+  const uint8_t* pw[4];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) px[q] = (const uint16_t*)p.x + min(m0 + row + 64 * q, p.M - 1) * p.ldx;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pw[i] = p.w + (int64_t)min(n0 + wrow + 32 * i, p.N - 1) * p.ldw + piece * 16;
+  Eight<T> v[2][4];
+  i32x4 w[4];
+  auto load = [&](int kb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = *(const i32x4*)(pw[i] + (int64_t)kb * 128);
+    // (pieces that reach over the row's end are read where the last whole one is, and shifted down when they are cut)
+#pragma unroll
+    for (int q = 0; q < 2; ++q)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) __builtin_memcpy(&v[q][j].v, px[q] + min(kb * 128 + l * 8 + 32 * j, p.K - 8), 16);
+  };
+  auto cut = [&](int buf, int kb) __attribute__((always_inline)) {
+    if ((kb + 1) * 128 > p.K) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int over = kb * 128 + l * 8 + 32 * j - (p.K - 8);      // columns behind the last
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+          if (over > 0) {
+            typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+            u64x2 t = __builtin_bit_cast(u64x2, v[q][j].v);
+            const int bits = 16 * over;
+            if (bits >= 128) t = (u64x2)0;
+            else if (bits >= 64) { t[0] = t[1] >> (bits - 64); t[1] = 0; }
+            else { t[0] = (t[0] >> bits) | (t[1] << (64 - bits)); t[1] >>= bits; }
+            v[q][j].v = __builtin_bit_cast(u16x8, t);
+          }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+      uint32_t m = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { const uint32_t a = v[q][j].amax(); m = a > m ? a : m; }
+      const BlockScale bs = block_scale<FX>(dpp_umax<0x4E>(dpp_umax<0xB1>(m)));
+      const int at = row + 64 * q;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) *(uint2*)&tiles[buf][at][((2 * j + (l >> 1)) ^ turn(at)) * 16 + (l & 1) * 8] = quant8<T, FX>(v[q][j], bs);
+      if (l == 0) se[buf][at] = bs.byte;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) *(i32x4*)&tiles[buf][128 + wrow + 32 * i][(piece ^ turn(wrow + 32 * i)) * 16] = w[i];
+  };
+  // scales of W as in k_fp8_nt
+  const uint8_t* pb[2];
+  uint32_t sb[2], nb[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) { pb[i] = p.sw + (int64_t)min(n0 + (wn * 2 + i) * 32 + r, p.N - 1) * p.ldsw + kb0; nb[i] = *(const uint32_t*)pb[i]; }
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+  int off[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) off[c] = r * 128 + (((4 * h + c) ^ turn(r)) * 16);
+  load(kb0);
+  cut(0, kb0);
+  if (kb0 + 1 < kb1) load(kb0 + 1);
+  __syncthreads();
+  for (int kb = kb0; kb < kb1; ++kb) {
+    const int buf = (kb - kb0) & 1;
+    if (((kb - kb0) & 3) == 0) {
+      const bool more = kb + 4 < kb1;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) { sb[i] = nb[i]; pb[i] += 4; if (more) nb[i] = *(const uint32_t*)pb[i]; }
+    }
+    const uint8_t *ta = &tiles[buf][wm * 64][0], *tb = &tiles[buf][128 + wn * 64][0];
+    int sa[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) sa[j] = se[buf][wm * 64 + 32 * j + r];
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks) {
+      i32x8 fa[2], fb[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        fb[i] = __builtin_shufflevector(*(const i32x4*)(tb + i * 4096 + off[2 * ks]), *(const i32x4*)(tb + i * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+        fa[i] = __builtin_shufflevector(*(const i32x4*)(ta + i * 4096 + off[2 * ks]), *(const i32x4*)(ta + i * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) acc[i][j] = mfma8<F8_E4M3, FX>(fb[i], fa[j], acc[i][j], (int)sb[i], sa[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) sb[i] >>= 8;
+    if (kb + 1 < kb1) {
+      cut(buf ^ 1, kb + 1);
+      if (kb + 2 < kb1) load(kb + 2);
+    }
+    __syncthreads();            // this tile has been read, the next one is written
+  }
+  Fp8Out o = p.o;
+  if (p.splits > 1) { o.y = (float*)o.y + (int64_t)blockIdx.y * p.M * p.N; o.ldy = p.N; o.type = FT_F32; o.relu = 0; }
+  uint8_t* buf = &tiles[0][0][0] + wave * 8192;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int64_t m = m0 + (wm * 2 + j) * 32;
+    if (o.type == FT_F32) store_block<true>(o, acc[0][j], acc[1][j], buf, m, p.M, n0 + wn * 64, p.N, lane);
+    else store_block<false>(o, acc[0][j], acc[1][j], buf, m, p.M, n0 + wn * 64, p.N, lane);
+  }
+}
+
 // ------------------------------------------------------------------------------------------------------ weight gradients
 // dW = G^T X over the rows of g and x, both cut into blocks of 128 ROWS per column on the way.  The result is fp32 and the sum long, so the
 // 8-bit values go back to bf16 (exactly) for the bf16 matrix instruction.  A block of 8 waves owns 64 NI x 256 results and a range of
@@ -866,22 +998,19 @@ extern "C" int aln_fp8_quantize_t(const void* x, int32_t x_type, int64_t ldx, in
 // and without parts: 256 x 512 x 4096 12.7 us and 24.2, 64 x 1024 x 4096 11.0 and 28.2, 1024 x 1024 x 4096 22.6 and 29.8; but 1920 x 1024 x 2048 in
 // four parts 26.4 and 15.6 in one.
 struct NtPlan { int splits, per; };
-static NtPlan nt_plan(int64_t M, int N, int64_t K) {
+static NtPlan nt_plan(int64_t M, int N, int64_t K, double step = 0.8) {
   const int64_t tiles = (M + 127) / 128 * ((N + 127) / 128), nkb = ceil128(K) / 128;
   NtPlan best{1, (int)((nkb + 3) / 4 * 4)};
-  double least = 0.8 * nkb;
-  for (int64_t s = 2; s * tiles <= 256 && 4 * s <= nkb; ++s) {
-    const int64_t per = ((nkb + s - 1) / s + 3) / 4 * 4, parts = (nkb + per - 1) / per;    // (whole words of scales)
-    const double t = 0.8 * per + 4.0 + 2e-6 * parts * M * N;
-    if (t < least) { least = t; best = {(int)parts, (int)per}; }
+  double least = step * nkb;
+  for (int64_t per = 4; per < nkb; per += 4) {            // (whole words of scales)
+    const int64_t parts = (nkb + per - 1) / per;
+    const double t = step * per + 4.0 + 2e-6 * parts * M * N;
+    if (parts * tiles <= 256 && t < least) { least = t; best = {(int)parts, (int)per}; }
   }
   return best;
 }
-extern "C" int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K) {
-  if (M <= 0 || N <= 0 || K <= 0) return 0;
-  const NtPlan pl = nt_plan(M, N, K);
-  return pl.splits > 1 ? (int64_t)pl.splits * M * N * 4 : 0;
-}
+static int64_t slab_bytes(const NtPlan& pl, int64_t M, int N) { return pl.splits > 1 ? (int64_t)pl.splits * M * N * 4 : 0; }
+extern "C" int64_t aln_fp8_nt_ws_bytes(int64_t M, int32_t N, int64_t K) { return M <= 0 || N <= 0 || K <= 0 ? 0 : slab_bytes(nt_plan(M, N, K), M, N); }
 template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI> static int nt_launch(const Fp8NT& p, hipStream_t st) {
   constexpr int BM = WM * MI * 32, BN = WN * NI * 32, LDS = 2 * (BM + BN) * 128;
   // (at every call: it holds for the current device)
@@ -926,18 +1055,33 @@ extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t
 }
 
 // ---- x W^T for x as it is.  16-bit x and y, e4m3 weights, up to 512 columns (1024 with few rows or few columns of y): the one-launch kernel;
-// otherwise blocks of x in the workspace, then the product.
+// otherwise, with few rows or few columns of y, the tiles that cut rows (lin_cut), or blocks of x in the workspace, then the product.
 // (eight waves hold 256 columns of y at 513 .. 1024 columns of x, and every further part cuts the rows again.  In one launch and in two: 64 x 1024 x 4096
 // 8.9 us and 14.0, 1024 x 1024 x 4096 16.9 and 16.6, 8192 x 1024 x 4096 62 and 50, 8192 x 640 x 4096 44 and 38, 8192 x 1024 x 1024 24 either way, 65537 x 1024
 // x 512 80 and 95; up to 512 columns 131072 x 512 x 4096 482 and 557)
 static bool lin_fused(int64_t M, int N, int64_t K, int x_type, int y_type, int fmt_w) {
   return (K <= 512 || (K <= 1024 && (N <= 1024 || M <= 512))) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
 }
+// Otherwise k_fp8_cut, where its column tiles are few or there are few rows to cut again: 444219 x 1203 x 40 283 us and 499 in two launches, 65536 x 1280
+// x 128 40 and 67, 200000 x 1100 x 300 251 and 294, 30000 x 4096 x 384 130 and 136, but x 512 154 and 143; 3 x 1844 x 3304 13.4 and 13.5 (a launch less on the
+// host: 13.4 and 15.4 a call), 300 x 2048 x 2048 19.7 and 21.5, but 1024 x 2048 x 1024 26.6 and 20.5.
+#define CUT_STEP 1.4                 // us of a lone block's step (nt_plan)
+static bool lin_cut(int64_t M, int N, int x_type, int y_type, int fmt_w) {
+  return (N <= 384 || M <= 384) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
+}
 static inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t x_type, int32_t y_type, int32_t fmt_w) {
   if (M <= 0 || N <= 0 || K <= 0 || lin_fused(M, N, K, x_type, y_type, fmt_w)) return 0;
+  if (lin_cut(M, N, x_type, y_type, fmt_w)) return slab_bytes(nt_plan(M, N, K, CUT_STEP), M, N);
   const int64_t nb = ceil128(K) / 128;
   return M * nb * 128 + up16(M * ((nb + 3) / 4 * 4)) + aln_fp8_nt_ws_bytes(M, N, K);
+}
+template <int T, int FX> static int cut_launch(const Fp8Cut& p, hipStream_t st) {
+  const int64_t g = (p.M + 127) / 128 * ((p.N + 127) / 128);
+  ALN_REQUIRE(g < (int64_t)1 << 22, "fp8_linear: %lld x %d results are too many for one launch", (long long)p.M, p.N);
+  hipLaunchKernelGGL((k_fp8_cut<T, FX>), dim3(xcd_grid(g), p.splits), dim3(256), 0, st, p);
+  ALN_CHECK_LAUNCH("fp8_linear");
+  return 0;
 }
 template <int T, int FX, int NKB> static int lin_launch(const Fp8Linear& p, hipStream_t st) {
   const int64_t g = (int64_t)p.ranges * p.parts;
@@ -969,6 +1113,19 @@ extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_
   const int64_t need = aln_fp8_linear_ws_bytes(M, N, K, x_type, y_type, fmt_w);
   ALN_REQUIRE(ws_bytes >= need && (need == 0 || (ws && ((uintptr_t)ws & 15) == 0)), "fp8_linear: the workspace needs %lld bytes, aligned to 16", (long long)need);
   const int nkb = (int)(ceil128(K) / 128);
+  if (!lin_fused(M, N, K, x_type, y_type, fmt_w) && lin_cut(M, N, x_type, y_type, fmt_w)) {
+    const NtPlan pl = nt_plan(M, N, K, CUT_STEP);
+    const Fp8Out o{y, ldy, y_type, relu};
+    Fp8Cut p{x, ldx, (const uint8_t*)w, ldw, sw, ldsw, M, N, K, nkb, pl.splits, pl.per, o};
+    if (pl.splits > 1) p.o.y = ws;
+    hipStream_t st = (hipStream_t)stream;
+    const int rc = x_type == FT_F16 ? (fmt_x == F8_E4M3 ? cut_launch<FT_F16, F8_E4M3>(p, st) : cut_launch<FT_F16, F8_E5M2>(p, st))
+                                    : (fmt_x == F8_E4M3 ? cut_launch<FT_BF16, F8_E4M3>(p, st) : cut_launch<FT_BF16, F8_E5M2>(p, st));
+    if (rc || pl.splits == 1) return rc;
+    hipLaunchKernelGGL(k_fp8_join, dim3(aln_grid_for((M * N + 3) / 4, 32, 4096)), dim3(256), 0, st, (const float*)ws, pl.splits, M, N, o);
+    ALN_CHECK_LAUNCH("fp8_linear");
+    return 0;
+  }
   if (!lin_fused(M, N, K, x_type, y_type, fmt_w)) {
     uint8_t* q = (uint8_t*)ws, *sc = q + M * nkb * 128, *rest = sc + up16(M * ((nkb + 3) / 4 * 4));
     const int rc = aln_fp8_quantize(x, x_type, ldx, M, K, fmt_x, q, (int64_t)nkb * 128, sc, (nkb + 3) / 4 * 4, stream);

@@ -188,9 +188,11 @@ def test_product_workspaces_follow_the_call():
     """No workspace where one launch does it; with one, room for the blocks of x and for the parts of a split contraction."""
     L = hip.lib()
     assert L.aln_fp8_linear_ws_bytes(1 << 20, 4096, 512, 0, 0, 0) == 0 and L.aln_fp8_linear_ws_bytes(1, 4096, 1024, 1, 0, 0) == 0
-    for sizes in ((1 << 20, 4096, 512, 2, 0, 0), (1 << 20, 4096, 512, 0, 2, 0), (1 << 20, 4096, 512, 0, 0, 1), (8192, 4096, 1024, 0, 0, 0), (1, 1, 1025, 0, 0, 0)):
+    for sizes in ((1 << 20, 4096, 512, 2, 0, 0), (1 << 20, 4096, 512, 0, 2, 0), (1 << 20, 4096, 512, 0, 0, 1), (8192, 4096, 1024, 0, 0, 0), (1000, 1000, 1025, 0, 0, 0)):
         m, n, k = sizes[:3]
         assert L.aln_fp8_linear_ws_bytes(*sizes) >= m * -(-k // 128) * 129 + L.aln_fp8_nt_ws_bytes(m, n, k)
+    for m, n, k in ((1, 1, 1025), (3, 3304, 1844), (1 << 19, 40, 1203)):        # rows cut on the way: room for parts alone
+        assert L.aln_fp8_linear_ws_bytes(m, n, k, 0, 1, 0) % (4 * m * n) == 0
     for m, n, k in ((1, 1, 1), (1003, 130, 77), (1 << 19, 512, 512), (43200, 128, 512)):
         assert L.aln_fp8_grad_weight_ws_bytes(m, n, k, 0, 0) % (4 * n * k) == 0
         assert L.aln_fp8_grad_weight_ws_bytes(m, n, k, 2, 0) >= (n + k) * -(-m // 128) * 129

@@ -467,3 +467,35 @@ def test_linear_out_tells_autograd(fp8):
     with torch.inference_mode():
         o = torch.empty(5, 64, device='cuda')
         assert torch.equal(fp8.linear(x, w, out=o), x)
+
+
+@pytest.mark.parametrize('fmt', ['e4m3', 'e5m2'])
+@pytest.mark.parametrize('dtype', [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize('M,K,N', [(1, 1025, 5), (1, 1086, 1059), (130, 1033, 384), (385, 1100, 384), (385, 1100, 385), (384, 1151, 400), (128, 2048, 128), (5, 4095, 129),
+                                   (3000, 1153, 40)])
+def test_linear_rows_cut_on_the_way_to_tiles(fp8, M, K, N, dtype, fmt):
+    """More columns than registers hold, few rows or few columns of results: x a view between NaN columns, its last piece of any length."""
+    g = torch.Generator().manual_seed(M + K + N)
+    x = (torch.randn(M, K, generator=g) * torch.rand(M, 1, generator=g)).to(dtype)
+    w = torch.randn(N, K, generator=g) / math.sqrt(K)
+    wide = torch.full((M, K + 11), math.nan, dtype=dtype, device='cuda')
+    wide[:, 3:3 + K] = x.cuda()
+    want, tol = product_bound(blocks64(x, fmt)[0], blocks64(w, 'e4m3')[0], K, dtype)
+    ws = fp8.quantize(w.cuda())
+    got = fp8.linear(wide[:, 3:3 + K], ws, fmt=fmt)
+    check(got, want, tol)
+    assert torch.equal(got, fp8.linear(x.cuda(), ws, fmt=fmt))
+
+
+def test_linear_cut_rows_nonfinite_and_broadcast(fp8):
+    g = torch.Generator().manual_seed(0)
+    x, w = torch.randn(200, 1300, generator=g).half(), torch.randn(300, 1300, generator=g) / 36
+    sq = fp8.quantize(w.cuda())
+    clean = fp8.linear(x.cuda(), sq)
+    bad = x.clone()
+    bad[7, 1299], bad[150, 0], bad[151, 700] = math.nan, math.inf, -math.inf
+    got, rows = fp8.linear(bad.cuda(), sq), [7, 150, 151]
+    keep = [i for i in range(200) if i not in rows]
+    assert torch.isnan(got[rows]).all() and torch.equal(got[keep], clean[keep])
+    one = x[:1].cuda().expand(200, 1300)
+    assert torch.equal(fp8.linear(one, sq), fp8.linear(one.contiguous(), sq))
