@@ -38,7 +38,7 @@ _PLAIN = {torch.Tensor, torch.nn.Parameter}
 _dtype = operator.attrgetter('dtype')
 
 
-def _check(name, grads, out, loss_scale, found_inf):
+def _check(name, grads, out, loss_scale, found_inf, norm):
     """Say what is wrong with the arguments (the slow way: one is known to be)."""
     dev = getattr(grads[0], 'device', None)
     for i, t in enumerate(grads):
@@ -51,14 +51,14 @@ def _check(name, grads, out, loss_scale, found_inf):
     for i, (t, o) in enumerate(zip(grads, out or ())):
         if not torch.is_tensor(o) or o.dtype != t.dtype or o.shape != t.shape or o.device != dev or (o.stride() != t.stride() and not (o.is_contiguous() and t.is_contiguous())):
             raise ValueError(f'{name}: output {i} must have the type, shape, strides and device of its tensor')
-    for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32)):
+    for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32), ('norm', norm, torch.float32)):
         if w is not None and (not torch.is_tensor(w) or w.dtype != dt or w.numel() < 1 or w.device != dev):
             raise ValueError(f'{name}: {what} must be a device tensor of {dt} beside the gradients')
     if dev.type != 'cuda':
         raise ValueError(f'{name}: autolabel_amd.clip has no CPU path: needs device tensors')
 
 
-def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
+def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf, norm):
     grads = [grads] if torch.is_tensor(grads) else list(grads)
     n = len(grads)
     if not n:
@@ -74,12 +74,13 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
         same = out is None or all(map(_T.is_same_size, out, grads))
         if len(device) == 1 and len(types) == 1 and min(device) >= 0 and types <= TYPES.keys() and same:
             codes = array.array('i', (TYPES[types.pop()],)) * n
-    if codes is None or loss_scale is not None or found_inf is not None:
-        _check(name, grads, out, loss_scale, found_inf)
+    if codes is None or loss_scale is not None or found_inf is not None or norm is not None:
+        _check(name, grads, out, loss_scale, found_inf, norm)
         codes = array.array('i', [TYPES[t.dtype] for t in grads])
     dev = grads[0].device
     with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
+        if norm is None:
+            norm = torch.empty((), dtype=torch.float32, device=dev)
         ws = torch.empty(H.lib().aln_grad_clip_ws_bytes(n), dtype=torch.uint8, device=dev)
         g, o = array.array('Q', map(_T.data_ptr, grads)), None if out is None else array.array('Q', map(_T.data_ptr, out))
         sizes = array.array('q', map(_T.numel, grads))
@@ -89,19 +90,20 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf):
     return norm
 
 
-def grad_norm(grads, loss_scale=None, found_inf=None):
+def grad_norm(grads, loss_scale=None, found_inf=None, norm=None):
     """sqrt of the sum of all squares of the tensors ``grads``, over ``loss_scale`` -> fp32 scalar on the device (squares and sums in fp64;
-    the same bits on every call).  ``found_inf`` (int32, device) is set to 1 when the norm is not finite."""
-    return _launch('grad_norm', grads, 0.0, False, None, loss_scale, found_inf)
+    the same bits on every call).  ``found_inf`` (int32, device) is set to 1 when the norm is not finite.  ``norm``: an fp32 tensor on the device
+    to write the norm into and return (one that a captured graph and eager calls share, say)."""
+    return _launch('grad_norm', grads, 0.0, False, None, loss_scale, found_inf, norm)
 
 
-def clip_grad_norm_(grads, max_norm, out=None, loss_scale=None, found_inf=None):
+def clip_grad_norm_(grads, max_norm, out=None, loss_scale=None, found_inf=None, norm=None):
     """Scale the tensors ``grads`` by min(1, max_norm / (norm + 1e-6)), in place or into ``out``, and return their ``grad_norm``.
 
     The tensors may differ in type (fp16, bf16, fp32) and size; no two may share memory.  Gradients that a loss scaler has multiplied keep
     its factor: ``loss_scale`` (fp32, device) only divides the norm.  A norm that is not finite scales nothing (``out`` is then a copy) and
-    sets ``found_inf``: the caller skips that step."""
+    sets ``found_inf``: the caller skips that step.  ``norm`` as in ``grad_norm``."""
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError(f'clip_grad_norm_: max_norm = {max_norm}')
-    return _launch('clip_grad_norm_', grads, max_norm, True, out, loss_scale, found_inf)
+    return _launch('clip_grad_norm_', grads, max_norm, True, out, loss_scale, found_inf, norm)

@@ -27,8 +27,10 @@ class TrainEngine:
         if max_grad_norm is not None and shard_optimizer:
             raise ValueError('TrainEngine: max_grad_norm needs every rank to hold the whole gradient (shard_optimizer leaves it 1 / world of the table\'s)')
         self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
-        self.grad_norm = None    # fp32 scalar on the device: the norm of the last clipped step, before clipping
         self.pipe, self.P, self.L = pipe, pipe.P, pipe.L
+        # fp32 scalar on the device: the norm of the last clipped step, before clipping (0 before the first; None without clipping).  One buffer for the
+        # engine's life: eager steps and every captured graph write the same
+        self.grad_norm = None if self.max_grad_norm is None else torch.zeros((), dtype=torch.float32, device=self.P.device)
         # hash-grid levels per scatter launch / gradient bucket of the overlapped exchange (level_groups).  Resolved ONCE, here: an explicit
         # argument wins; ALN_LEVEL_GROUP is only the default for level_group=None (re-reading the environment on every call let the
         # variable override the argument, and ranks with different environments would issue different collective sequences)
@@ -276,7 +278,7 @@ class TrainEngine:
         a norm that is not finite raises the step's overflow flag, and the optimizer skips the step and backs the scale off."""
         if self.max_grad_norm is not None:
             from .clip import clip_grad_norm_
-            self.grad_norm = clip_grad_norm_(self.P.grad[:self.L.n_total], self.max_grad_norm, loss_scale=self.state_f[0:1], found_inf=self.state_i[2:3])
+            clip_grad_norm_(self.P.grad[:self.L.n_total], self.max_grad_norm, loss_scale=self.state_f[0:1], found_inf=self.state_i[2:3], norm=self.grad_norm)
 
     def optimizer_step(self, step_dev=None, skip_grid=False):
         P, L, sc = self.P, self.L, self.scaler_cfg
