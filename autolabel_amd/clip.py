@@ -36,6 +36,15 @@ def _dense(t):
 _T = torch.Tensor
 _PLAIN = {torch.Tensor, torch.nn.Parameter}
 _dtype = operator.attrgetter('dtype')
+_requires_grad = operator.attrgetter('requires_grad')
+
+
+def _check_tracked(name, grads, out, apply):
+    """Some tensor requires a gradient: refuse what autograd would not see, and parameters handed over in place of their gradients."""
+    if torch.is_grad_enabled():
+        raise ValueError(f'{name}: a tensor requires a gradient, and autograd does not see what is done here: pass the parameters\' .grad, or call under torch.no_grad()')
+    if apply and any(o is t and torch.is_tensor(t) and t.requires_grad and t.is_leaf for t, o in zip(grads, grads if out is None else out)):
+        raise ValueError(f'{name}: a tensor requires a gradient: it is a parameter, not one\'s gradient (pass the parameters\' .grad)')
 
 
 def _check(name, grads, out, loss_scale, found_inf, norm):
@@ -69,7 +78,10 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf, norm):
             raise ValueError(f'{name}: {n} tensors, {len(out)} outputs')
     every = grads if out is None else grads + out
     codes = None                 # the tensors' types, where the quick checks already tell
-    if set(map(type, every)) <= _PLAIN and all(map(_T.is_contiguous, every)):
+    plain = set(map(type, every)) <= _PLAIN
+    if any(map(_requires_grad, every)) if plain else any(getattr(t, 'requires_grad', False) for t in every):
+        _check_tracked(name, grads, out, apply)
+    if plain and all(map(_T.is_contiguous, every)):
         device, types = set(map(_T.get_device, every)), set(map(_dtype, every))
         same = out is None or all(map(_T.is_same_size, out, grads))
         if len(device) == 1 and len(types) == 1 and min(device) >= 0 and types <= TYPES.keys() and same:
@@ -87,13 +99,16 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf, norm):
         H.call('aln_grad_clip', n, g.buffer_info()[0], None if o is None else o.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], max_norm,
                int(apply), loss_scale.data_ptr() if loss_scale is not None else None, norm.data_ptr(),
                found_inf.data_ptr() if found_inf is not None else None, ws.data_ptr(), ws.numel(), H.raw_stream())
+    if apply:           # (a backward pass that saved one of them notices; inference tensors have no version)
+        torch.autograd.graph.increment_version(grads if out is None else out)
     return norm
 
 
 def grad_norm(grads, loss_scale=None, found_inf=None, norm=None):
     """sqrt of the sum of all squares of the tensors ``grads``, over ``loss_scale`` -> fp32 scalar on the device (squares and sums in fp64;
     the same bits on every call).  ``found_inf`` (int32, device) is set to 1 when the norm is not finite.  ``norm``: an fp32 tensor on the device
-    to write the norm into and return (one that a captured graph and eager calls share, say)."""
+    to write the norm into and return (one that a captured graph and eager calls share, say).  Not differentiable: while gradients are tracked,
+    tensors that require one are refused."""
     return _launch('grad_norm', grads, 0.0, False, None, loss_scale, found_inf, norm)
 
 
@@ -102,7 +117,10 @@ def clip_grad_norm_(grads, max_norm, out=None, loss_scale=None, found_inf=None, 
 
     The tensors may differ in type (fp16, bf16, fp32) and size; no two may share memory.  Gradients that a loss scaler has multiplied keep
     its factor: ``loss_scale`` (fp32, device) only divides the norm.  A norm that is not finite scales nothing (``out`` is then a copy) and
-    sets ``found_inf``: the caller skips that step.  ``norm`` as in ``grad_norm``."""
+    sets ``found_inf``: the caller skips that step.  ``norm`` as in ``grad_norm``.
+
+    Unlike torch.nn.utils.clip_grad_norm_ this takes the gradients, not the parameters: a leaf that requires a gradient is never scaled in place.
+    As for ``grad_norm``, tensors that require one are refused while gradients are tracked; what is written counts as modified in place."""
     max_norm = float(max_norm)
     if math.isnan(max_norm) or max_norm < 0:
         raise ValueError(f'clip_grad_norm_: max_norm = {max_norm}')
