@@ -333,9 +333,9 @@ class SimpleTrainer(Trainer):
                 with torch.autocast('cuda', enabled=self.fp16):
                     _, _, loss = self.train_step(data)
                 self.scaler.scale(loss).backward()
-                self._clip_gradients()
-                for opt in self.optimizers:
-                    self.scaler.step(opt)
+                if self._clip_gradients():
+                    for opt in self.optimizers:
+                        self.scaler.step(opt)
                 self.scaler.update()
                 if hasattr(bar, 'set_description'):
                     bar.set_description(f'Loss: {loss:.04f}')
@@ -345,15 +345,20 @@ class SimpleTrainer(Trainer):
         self._step_scheduler(loss)
 
     def _clip_gradients(self):
-        """Generic loop: unscale the optimizers' gradients (GradScaler.step then does not again) and clip their global norm."""
+        """Generic loop: unscale the optimizers' gradients (GradScaler.step then does not again) and clip their global norm.  False: the norm is not
+        finite -- a gradient is not, or the norm of finite ones is beyond fp32, which the scaler's own check lets pass -- so nothing was clipped and
+        the step is to be skipped (the host waits for that flag, as GradScaler.step does for its own)."""
         if self.max_grad_norm is None:
-            return
+            return True
         from .clip import clip_grad_norm_
         for opt in self.optimizers:
             self.scaler.unscale_(opt)
         grads = [p.grad for opt in self.optimizers for g in opt.param_groups for p in g['params'] if p.grad is not None]
-        if grads:
-            clip_grad_norm_(grads, self.max_grad_norm)
+        if not grads:
+            return True
+        flag = torch.zeros(1, dtype=torch.int32, device=grads[0].device)
+        clip_grad_norm_(grads, self.max_grad_norm, found_inf=flag)
+        return not flag.item()
 
     def fused_step(self, data):
         eng = self._engine()
@@ -517,8 +522,8 @@ class InteractiveTrainer(SimpleTrainer):
             with torch.autocast('cuda', enabled=self.fp16):
                 _, _, loss = self.train_step(data)
             self.scaler.scale(loss).backward()
-            self._clip_gradients()
-            self.scaler.step(self.optimizer)
+            if self._clip_gradients():
+                self.scaler.step(self.optimizer)
             self.scaler.update()
         self.step += 1
         self.global_step += 1
