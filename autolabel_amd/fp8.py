@@ -119,7 +119,7 @@ def _empty_blocks(rows, cols, fmt, device):
 
 def quantize(x, fmt='e4m3', transpose=False):
     """Blocks of ``x`` [..., K] along its last axis -> Fp8Blocks of [rows, K]; ``transpose=True``: blocks of x^T along the rows of x ->
-    Fp8Blocks of [K, rows] (what a product over the rows needs)."""
+    Fp8Blocks of [K, rows] (what a product over the rows needs).  Blocks carry no gradient."""
     _need(fmt in FORMATS, f'quantize: unknown 8-bit format {fmt!r} (one of {", ".join(FORMATS)})')
     x = _rows('quantize', x)
     m, k = x.shape
@@ -155,7 +155,14 @@ def matmul(a, b, out_dtype=torch.float16, relu=False):
 def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
     """x [..., K] W^T for ``weight`` = Fp8Blocks of W [N, K] -> [..., N] of x's type (or ``out_dtype``); the rows of x are cut into blocks of
     ``fmt`` on the way.  ``relu``: negative results become 0.  ``out``: a contiguous tensor of the result's shape to write it into (its type
-    decides the result's); it must not overlap x."""
+    decides the result's); it must not overlap x.  The result carries no gradient: while gradients are tracked, an x that requires one is refused
+    (``Linear`` is the layer with its gradients)."""
+    if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():
+        raise ValueError('linear: x requires a gradient, which the result would not carry: use fp8.Linear, x.detach(), or call under torch.no_grad()')
+    return _linear(x, weight, relu, out_dtype, fmt, out)
+
+
+def _linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
     if not isinstance(weight, Fp8Blocks):
         raise ValueError('linear: weight must be Fp8Blocks (fp8.quantize)')
     weight._check('linear: weight')
@@ -194,7 +201,8 @@ def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
 def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True):
     """Gradients of y = x W^T (no activation) from ``g`` = dL/dy [..., N] and ``x`` [..., K]: (dL/dx of x's type, dL/dW [N, K] fp32), either
     one None where not needed.  ``weight_t`` = Fp8Blocks of W^T [K, N] (not read for dL/dW alone: may be None then).  g is cut into blocks of
-    ``grad_fmt`` along N for dL/dx, g and x along their rows for dL/dW; the sums over the rows are taken in a fixed order."""
+    ``grad_fmt`` along N for dL/dx, g and x along their rows for dL/dW; the sums over the rows are taken in a fixed order.  The gradients are not
+    tracked themselves (no second derivatives)."""
     if grad_fmt not in FORMATS:
         raise ValueError(f'linear_backward: unknown 8-bit format {grad_fmt!r} (one of {", ".join(FORMATS)})')
     gr, xr = _rows('linear_backward: g', g), _rows('linear_backward: x', x)
@@ -208,7 +216,7 @@ def linear_backward(g, x, weight_t, grad_fmt='e4m3', need_dx=True, need_dw=True)
         weight_t._check('linear_backward: weight_t')
         if weight_t.rows != k or weight_t.cols != n:
             raise ValueError(f'linear_backward: weight_t is {weight_t.rows} x {weight_t.cols}, x has {k} columns and g {n}')
-        dx = linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt)
+        dx = _linear(gr, weight_t, out_dtype=x.dtype, fmt=grad_fmt)
         if len(x.shape) != 2:
             dx = dx.reshape(x.shape)
     if need_dw:
