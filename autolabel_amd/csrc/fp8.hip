@@ -949,6 +949,7 @@ __global__ __launch_bounds__(256) void k_fp8_join(const float* __restrict__ slab
 }
 
 // ------------------------------------------------------------------------------------------------------------ entry points
+#define MOST32 (((int64_t)1 << 31) - 256)      // sizes that are counted in 32 bits, in tiles of up to 256
 static bool is_ft(int t) { return t >= FT_F16 && t <= FT_F32; }
 static bool is_f8(int f) { return f == F8_E4M3 || f == F8_E5M2; }
 static bool blocks_ok(const void* q, int64_t ldq, const void* s, int64_t lds, int64_t K) {
@@ -976,7 +977,7 @@ static int quant_fmt(int fmt, bool t, const void* x, int64_t ldx, int64_t M, int
 static int quantize(const char* name, bool t, const void* x, int x_type, int64_t ldx, int64_t M, int K, int fmt, void* q, int64_t ldq, uint8_t* scale, int64_t lds,
                     hipStream_t st) {
   ALN_REQUIRE(is_ft(x_type) && is_f8(fmt), "%s: unknown type %d or format %d", name, x_type, fmt);
-  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && K >= 1 && ldx >= 0, "%s: %lld x %d values with pitch %lld", name, (long long)M, K, (long long)ldx);
+  ALN_REQUIRE(M >= 0 && M <= MOST32 && K >= 1 && K <= MOST32 && ldx >= 0, "%s: %lld x %d values with pitch %lld", name, (long long)M, K, (long long)ldx);
   if (M == 0) return 0;
   ALN_REQUIRE(x, "%s: NULL pointer", name);
   ALN_REQUIRE(((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0, "%s: x is not aligned to its type", name);
@@ -1034,7 +1035,7 @@ extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t
                           int32_t fmt_b, int64_t M, int32_t N, int64_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws, int64_t ws_bytes,
                           void* stream) {
   ALN_REQUIRE(is_f8(fmt_a) && is_f8(fmt_b) && is_ft(y_type), "fp8_nt: unknown format %d, %d or type %d", fmt_a, fmt_b, y_type);
-  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && K < (int64_t)1 << 31 && ldy >= N, "fp8_nt: sizes %lld x %d x %lld, pitch %lld", (long long)M, N, (long long)K,
+  ALN_REQUIRE(M >= 0 && M <= MOST32 && N >= 1 && N <= MOST32 && K >= 1 && K <= MOST32 && ldy >= N, "fp8_nt: sizes %lld x %d x %lld, pitch %lld", (long long)M, N, (long long)K,
               (long long)ldy);
   if (M == 0) return 0;
   ALN_REQUIRE(blocks_ok(a, lda, sa, ldsa, K) && blocks_ok(b, ldb, sb, ldsb, K), FP8_BAD_BLOCKS, "fp8_nt");
@@ -1105,7 +1106,7 @@ template <int T, int FX> static int lin_pick(const Fp8Linear& p, int nkb, hipStr
 extern "C" int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, const void* w, int64_t ldw, const uint8_t* sw, int64_t ldsw, int32_t fmt_w,
                               int64_t M, int32_t N, int32_t K, void* y, int64_t ldy, int32_t y_type, int32_t relu, void* ws, int64_t ws_bytes, void* stream) {
   ALN_REQUIRE(is_ft(x_type) && is_ft(y_type) && is_f8(fmt_x) && is_f8(fmt_w), "fp8_linear: unknown type %d, %d or format %d, %d", x_type, y_type, fmt_x, fmt_w);
-  ALN_REQUIRE(M >= 0 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldx >= 0 && ldy >= N && ldx < 1 << 25 && ldy < 1 << 25,
+  ALN_REQUIRE(M >= 0 && M <= MOST32 && N >= 1 && K >= 1 && K <= MOST32 && ldx >= 0 && ldy >= N && ldx < 1 << 25 && ldy < 1 << 25,
               "fp8_linear: sizes %lld x %d x %d, pitches %lld, %lld (under 2^25)", (long long)M, N, K, (long long)ldx, (long long)ldy);
   if (M == 0) return 0;
   ALN_REQUIRE(blocks_ok(w, ldw, sw, ldsw, K), FP8_BAD_BLOCKS, "fp8_linear");
@@ -1196,7 +1197,7 @@ template <int T> static int tn_pick(const Fp8TN& p, const TnPlan& t, int fmt_g, 
 extern "C" int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, int32_t fmt_g, const void* x, int32_t x_type, int64_t ldx, int64_t M, int32_t N, int32_t K,
                                    float* dw, void* ws, int64_t ws_bytes, void* stream) {
   ALN_REQUIRE(is_ft(g_type) && is_ft(x_type) && is_f8(fmt_g), "fp8_grad_weight: unknown type %d, %d or format %d", g_type, x_type, fmt_g);
-  ALN_REQUIRE(M >= 1 && M < (int64_t)1 << 31 && N >= 1 && K >= 1 && ldg >= N && ldx >= K && ldg < 1 << 24 && ldx < 1 << 24,
+  ALN_REQUIRE(M >= 1 && M <= MOST32 && N >= 1 && K >= 1 && ldg >= N && ldx >= K && ldg < 1 << 24 && ldx < 1 << 24,
               "fp8_grad_weight: sizes %lld x %d x %d, pitches %lld, %lld (at least the columns, under 2^24)", (long long)M, N, K, (long long)ldg, (long long)ldx);
   ALN_REQUIRE(g && ((uintptr_t)g & (g_type == FT_F32 ? 3 : 1)) == 0 && x && ((uintptr_t)x & (x_type == FT_F32 ? 3 : 1)) == 0 && dw && ((uintptr_t)dw & 3) == 0,
               "fp8_grad_weight: g, x or dw is NULL or not aligned to its type");

@@ -23,6 +23,7 @@ from . import hip as H
 BLOCK = 128
 FORMATS = {'e4m3': (0, torch.float8_e4m3fn), 'e5m2': (1, torch.float8_e5m2)}
 TYPES = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}
+MOST = (1 << 31) - 256       # rows and columns (the C entry points count them, and tiles of them, in 32 bits)
 
 
 def _blocks(n):
@@ -58,6 +59,8 @@ class Fp8Blocks:
         words = s.shape
         if len(words) != 2 or s.dtype is not torch.uint8 or not s.is_contiguous() or words[0] != shape[0] or words[1] < nb or words[1] % 4 or s.get_device() != q.get_device():
             raise ValueError(f'{name}: scale must be contiguous uint8 [rows, a multiple of 4 >= {nb}] beside q, got {s.dtype} {tuple(s.shape)}')
+        if shape[0] > MOST or self.cols > MOST:
+            raise ValueError(f'{name}: {shape[0]} rows of {self.cols} columns: neither may be more than {MOST}')
 
 
 def _need(ok, message):
@@ -72,6 +75,8 @@ def _rows(name, x):
     shape = x.shape
     if not shape or not shape[-1]:
         raise ValueError(f'{name}: needs at least one column, got shape {tuple(shape)}')
+    if shape[-1] > MOST:
+        raise ValueError(f'{name}: {shape[-1]} columns are more than {MOST}')
     if len(shape) != 2:
         x = x.detach().reshape(-1, shape[-1])
     if x.stride(1) != 1 and shape[-1] > 1:

@@ -448,7 +448,7 @@ int aln_grad_pack_f16_clear(float* grad, int64_t n, int64_t n_pad, float mul, vo
 
 /* ---- products in 8-bit floating point, one power-of-two scale per block of 128 along the contracted axis (fp8.hip; no counterpart in
  * the reference, whose heads run in fp16).  Beside aln_wide_nt / aln_wide_tn for layers whose operands may be 8 bits wide.
- * Types (x_type, y_type): 0 fp16, 1 bf16, 2 fp32.  Formats (fmt): 0 e4m3 (largest 448), 1 e5m2 (largest 57344).
+ * Types (x_type, y_type): 0 fp16, 1 bf16, 2 fp32.  Formats (fmt): 0 e4m3 (largest 448), 1 e5m2 (largest 57344).  Rows and columns: up to 2^31 - 256.
  * A matrix [R, K] in blocks: q [R, ldq] bytes, ldq a multiple of 16 and >= 128 ceil(K / 128), zero behind column K; scale [R, lds] bytes
  * holding exponent + 127, lds a multiple of 4: x[r][k] ~ q[r][k] * 2^(scale[r][k / 128] - 127).  q 16-byte, scale 4-byte aligned.
  * aln_fp8_quantize: blocks of x [M, K], row pitch ldx elements (x aligned to its type only).  The scale is the smallest power of two
