@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void k_grad_sumsq(ClipList l, double* part) {
 
 // NT: what goes to another buffer passes the caches by, so that the gradients just squared are still there (36 -> 33 us for the 14.8 M
 // parameters of a field with 512-wide heads).
-template <int T, bool NT> __device__ inline void scale_chunk(const void* g, void* o, int64_t lo, int64_t hi, float f) {
+template <int T, bool NT> __device__ inline void scale_chunk(const void* g, void* o, int64_t lo, int64_t hi, float f, float p2) {
   typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
   typedef unsigned short u16x8u __attribute__((ext_vector_type(8), aligned(2)));
   int64_t i = lo + threadIdx.x * 8;
@@ -96,25 +96,27 @@ template <int T, bool NT> __device__ inline void scale_chunk(const void* g, void
   for (; i + 8 <= hi; i += 2048) {
     float v[8];
     load8<T>(g, i, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = v[j] * f * p2;
     if constexpr (T == FT_F32) {
-      const f32x4u a = {v[0] * f, v[1] * f, v[2] * f, v[3] * f}, b = {v[4] * f, v[5] * f, v[6] * f, v[7] * f};
+      const f32x4u a = {v[0], v[1], v[2], v[3]}, b = {v[4], v[5], v[6], v[7]};
       f32x4u* p = (f32x4u*)((float*)o + i);
       if (NT) { __builtin_nontemporal_store(a, p); __builtin_nontemporal_store(b, p + 1); }
       else { p[0] = a; p[1] = b; }
     } else {
       u16x8u w;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = T == FT_F16 ? __builtin_bit_cast(uint16_t, (h16)(v[j] * f)) : __builtin_bit_cast(uint16_t, (__bf16)(v[j] * f));
+      for (int j = 0; j < 8; ++j) w[j] = T == FT_F16 ? __builtin_bit_cast(uint16_t, (h16)v[j]) : __builtin_bit_cast(uint16_t, (__bf16)v[j]);
       u16x8u* p = (u16x8u*)((uint16_t*)o + i);
       if (NT) __builtin_nontemporal_store(w, p);
       else *p = w;
     }
   }
-  if (i < hi) for (; i < hi; ++i) store1<T>(o, i, load1<T>(g, i) * f);
+  if (i < hi) for (; i < hi; ++i) store1<T>(o, i, load1<T>(g, i) * f * p2);
 }
-template <int T> __device__ inline void scale_chunk(const void* g, void* o, int64_t lo, int64_t hi, float f) {
-  if (g == o) scale_chunk<T, false>(g, o, lo, hi, f);
-  else scale_chunk<T, true>(g, o, lo, hi, f);
+template <int T> __device__ inline void scale_chunk(const void* g, void* o, int64_t lo, int64_t hi, float f, float p2) {
+  if (g == o) scale_chunk<T, false>(g, o, lo, hi, f, p2);
+  else scale_chunk<T, true>(g, o, lo, hi, f, p2);
 }
 __global__ __launch_bounds__(256) void k_grad_scale(ClipList l, ClipRule r, int apply, int in_place) {
   __shared__ double lds4[4];
@@ -125,21 +127,24 @@ __global__ __launch_bounds__(256) void k_grad_scale(ClipList l, ClipRule r, int 
   if (r.loss_scale) norm /= (double)*r.loss_scale;
   const bool finite = fabs(norm) <= 3.4028234663852886e38;
   // a norm that is not finite scales nothing: the caller skips the step (found_inf), and the gradients show where it came from
-  const float f = finite ? (float)fmin(1.0, (double)r.max_norm / (norm + 1e-6)) : 1.f;
+  const double ratio = finite ? fmin(1.0, (double)r.max_norm / (norm + 1e-6)) : 1.0;
+  // (a factor near or under fp32's least normal keeps its bits as f 2^-100: v f does not overflow, f <= 1, and the power of two is exact)
+  const bool low = ratio < 0x1p-100;
+  const float f = (float)(low ? ratio * 0x1p100 : ratio), p2 = low ? 0x1p-100f : 1.f;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     if (r.norm) *r.norm = (float)norm;
     if (r.found_inf && !finite) *r.found_inf = 1;
   }
-  if (!apply || (in_place && f == 1.f)) return;
+  if (!apply || (in_place && f == 1.f && !low)) return;
   // backwards: what was squared last is the likeliest to be in the caches still
   const int total = l.first[l.count], grid = gridDim.x;
   for (int c = (total - 1) / grid * grid + (int)blockIdx.x; c >= 0; c -= grid) {
     if (c >= total) continue;
     const int k = clip_find(l, c);
     const int64_t lo = (int64_t)(c - l.first[k]) * CLIP_CHUNK, hi = min(lo + CLIP_CHUNK, l.n[k]);
-    if (l.type[k] == FT_F32) scale_chunk<FT_F32>(l.g[k], l.o[k], lo, hi, f);
-    else if (l.type[k] == FT_F16) scale_chunk<FT_F16>(l.g[k], l.o[k], lo, hi, f);
-    else scale_chunk<FT_BF16>(l.g[k], l.o[k], lo, hi, f);
+    if (l.type[k] == FT_F32) scale_chunk<FT_F32>(l.g[k], l.o[k], lo, hi, f, p2);
+    else if (l.type[k] == FT_F16) scale_chunk<FT_F16>(l.g[k], l.o[k], lo, hi, f, p2);
+    else scale_chunk<FT_BF16>(l.g[k], l.o[k], lo, hi, f, p2);
   }
 }
 
