@@ -11,12 +11,13 @@
 // That instruction accumulates in fp32, but aligns the 64 products of a step to the largest of them and drops what lies 13 binades below it
 // (measured; the older v_mfma_f32_32x32x16_fp8_fp8 does the same): 1.3e-5 of the result for Gaussian operands, 7e-5 for values spread over 12
 // binades.  Under the half step of a 16-bit result (4.9e-4, 3.9e-3), far above that of an fp32 one: products with an fp32 result turn the 8-bit
-// values back into bf16, which holds q 2^e exactly, and use the bf16 instruction (5e-8, at half the rate).
+// values back into bf16, which holds q 2^e exactly but at the ends of the exponents (WIDE_LO), and use the bf16 instruction (5e-8, at half the rate).
 // A block that holds an infinity or a NaN is NaN throughout (its row of the product would be non-finite in every column anyway).
 //
 // Layout: q [rows, ldq] bytes, columns [K, 128 ceil(K / 128)) zero; scale [rows, lds] bytes e + 127, lds a multiple of 4, so that the four
 // scales of 512 columns are one aligned 4-byte word.
 #include "common.h"
+#include <type_traits>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
@@ -230,7 +231,7 @@ template <int FA, int FB, int SA = 0, int SB = 0> __device__ inline f32x16 mfma8
   return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, FA, FB, SA, sa, SB, sb);
 }
 
-// two 8-bit values (the upper two of the word with HI) times a power of two, exact in bf16
+// two 8-bit values (the upper two of the word with HI) times a power of two, exact in bf16 between WIDE_LO and WIDE_HI
 typedef __bf16 b16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 b16x8 __attribute__((ext_vector_type(8)));
 template <int FMT, bool HI> __device__ inline b16x2 widen2(uint32_t w, float s) {
@@ -241,6 +242,18 @@ template <int FMT> __device__ inline b16x8 widen8(uint32_t w0, uint32_t w1, floa
   const b16x2 a = widen2<FMT, false>(w0, s), b = widen2<FMT, true>(w0, s), c = widen2<FMT, false>(w1, s), d = widen2<FMT, true>(w1, s);
   return (b16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
+
+// bf16 holds q 2^e exactly from 2^-133 up and under 2^128: for every q of a block with e between these (as e + 127).  The few scales outside, where a value
+// may be as small as 2^-135 (e4m3; e5m2 2^-142) or be 2^128, would lose bits, or become infinite and with a zero NaN.  Their powers of two are moved by
+// 2^16 from one operand to the other, which then holds what it can hold of the product: below 2^-149 there is nothing to lose.
+template <int FMT> constexpr uint32_t WIDE_LO = FMT == F8_E4M3 ? 3 : 10;
+template <int FMT> constexpr uint32_t WIDE_HI = FMT == F8_E4M3 ? 246 : 239;
+template <int FMT> __device__ inline int wide_end(uint32_t e) { return e < WIDE_LO<FMT> ? 1 : e > WIDE_HI<FMT> ? 2 : 0; }     // 1: small, 2: large
+// how an operand of kind c is moved beside one of kind d.  Two small ones' product is 0 however they are moved; two large ones', where it is not 0,
+// is infinite also 2^32 lower
+__device__ inline int wide_shift(int c, int d) { return c == 2 ? -16 : c == 1 ? 16 : d == 2 ? 16 : d == 1 ? -16 : 0; }
+// (at the ends of the range the product is infinite, or 0, all the same)
+template <int FMT> __device__ inline uint32_t wide_moved(uint32_t e, int by) { return (uint32_t)min(max((int)e + by, 1), (int)WIDE_HI<FMT>); }
 
 __device__ inline float relu_nan(float v) { return __builtin_elementwise_maximum(v, 0.f); }     // a NaN stays one
 
@@ -373,8 +386,7 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
   for (int c = 0; c < 4; ++c) off[c] = r * 128 + (((4 * h + c) ^ turn(r)) * 16);
   fetch(0);
   __syncthreads();
-  for (int kb = kb0; kb < kb1; ++kb) {
-    const int buf = (kb - kb0) & 1;
+  auto words = [&](int kb) __attribute__((always_inline)) {
     if (((kb - kb0) & 3) == 0) {
       const bool more = kb + 4 < kb1;
 #pragma unroll
@@ -382,43 +394,96 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
 #pragma unroll
       for (int i = 0; i < NI; ++i) { sb[i] = nb[i]; if (more) { pb[i] += 4; nb[i] = *(const uint32_t*)pb[i]; } }
     }
-    if (kb + 1 < kb1) fetch(buf ^ 1);
+  };
+  auto fragments = [&](int buf, int ks, i32x8 (&fa)[MI], i32x8 (&fb)[NI]) __attribute__((always_inline)) {
     const uint8_t *ta = smem8 + buf * ROWS * 128 + wm * MI * 4096, *tb = smem8 + buf * ROWS * 128 + BM * 128 + wn * NI * 4096;
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      fb[i] = __builtin_shufflevector(*(const i32x4*)(tb + i * 4096 + off[2 * ks]), *(const i32x4*)(tb + i * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+    for (int j = 0; j < MI; ++j)
+      fa[j] = __builtin_shufflevector(*(const i32x4*)(ta + j * 4096 + off[2 * ks]), *(const i32x4*)(ta + j * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
+  };
+  auto widened = [&](const i32x8 (&fa)[MI], const i32x8 (&fb)[NI], const uint32_t (&ea)[MI], const uint32_t (&eb)[NI]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      b16x8 xa[MI];
+#pragma unroll
+      for (int j = 0; j < MI; ++j) xa[j] = widen8<FA>(fa[j][2 * q], fa[j][2 * q + 1], __uint_as_float(ea[j] << 23));
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const b16x8 xb = widen8<FB>(fb[i][2 * q], fb[i][2 * q + 1], __uint_as_float(eb[i] << 23));
+#pragma unroll
+        for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb, xa[j], acc[i][j], 0, 0, 0);
+      }
+    }
+  };
+  auto finish = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < MI; ++j) sa[j] >>= 8;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) sb[i] >>= 8;
+    __syncthreads();            // the tile has been read, the next one has landed
+  };
+  int kb = kb0;
+  for (; kb < kb1; ++kb) {
+    const int buf = (kb - kb0) & 1;
+    words(kb);
+    uint32_t ea[MI], eb[NI];
+    if constexpr (WIDE) {
+      bool ends = false;
+#pragma unroll
+      for (int j = 0; j < MI; ++j) { ea[j] = sa[j] & 255u; ends |= wide_end<FA>(ea[j]) != 0; }
+#pragma unroll
+      for (int i = 0; i < NI; ++i) { eb[i] = sb[i] & 255u; ends |= wide_end<FB>(eb[i]) != 0; }
+      if (__any(ends)) break;
+    }
+    if (kb + 1 < kb1) fetch(buf ^ 1);
 #pragma unroll
     for (int ks = 0; ks < 2; ++ks) {
       i32x8 fa[MI], fb[NI];
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-        fb[i] = __builtin_shufflevector(*(const i32x4*)(tb + i * 4096 + off[2 * ks]), *(const i32x4*)(tb + i * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-      for (int j = 0; j < MI; ++j)
-        fa[j] = __builtin_shufflevector(*(const i32x4*)(ta + j * 4096 + off[2 * ks]), *(const i32x4*)(ta + j * 4096 + off[2 * ks + 1]), 0, 1, 2, 3, 4, 5, 6, 7);
-      if constexpr (WIDE) {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          b16x8 xa[MI];
-#pragma unroll
-          for (int j = 0; j < MI; ++j) xa[j] = widen8<FA>(fa[j][2 * q], fa[j][2 * q + 1], __uint_as_float((sa[j] & 255u) << 23));
-#pragma unroll
-          for (int i = 0; i < NI; ++i) {
-            const b16x8 xb = widen8<FB>(fb[i][2 * q], fb[i][2 * q + 1], __uint_as_float((sb[i] & 255u) << 23));
-#pragma unroll
-            for (int j = 0; j < MI; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb, xa[j], acc[i][j], 0, 0, 0);
-          }
-        }
-      } else {
+      fragments(buf, ks, fa, fb);
+      if constexpr (WIDE) widened(fa, fb, ea, eb);
+      else {
 #pragma unroll
         for (int j = 0; j < MI; ++j)
 #pragma unroll
           for (int i = 0; i < NI; ++i) acc[i][j] = mfma8<FB, FA>(fb[i], fa[j], acc[i][j], (int)sb[i], (int)sa[j]);
       }
     }
-#pragma unroll
-    for (int j = 0; j < MI; ++j) sa[j] >>= 8;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) sb[i] >>= 8;
-    __syncthreads();            // the tile has been read, the next one has landed
+    finish();
   }
+  // from a wave's first step with a scale at the ends of the exponents on: each kind of row with each kind of column in turn, the others as zeros (one
+  // barrier to a step here too: the waves of a block need not be in the same loop)
+  if constexpr (WIDE)
+    for (bool first = true; kb < kb1; ++kb, first = false) {
+      const int buf = (kb - kb0) & 1;
+      if (!first) words(kb);
+      if (kb + 1 < kb1) fetch(buf ^ 1);
+#pragma unroll 1
+      for (int pass = 0; pass < 9; ++pass) {
+        const int ca = pass / 3, cb = pass % 3, da = wide_shift(ca, cb), db = wide_shift(cb, ca);
+        uint32_t ea[MI], eb[NI];
+        bool ka[MI], kc[NI], any_a = false, any_b = false;
+#pragma unroll
+        for (int j = 0; j < MI; ++j) { ka[j] = wide_end<FA>(sa[j] & 255u) == ca; any_a |= ka[j]; ea[j] = wide_moved<FA>(sa[j] & 255u, da); }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) { kc[i] = wide_end<FB>(sb[i] & 255u) == cb; any_b |= kc[i]; eb[i] = wide_moved<FB>(sb[i] & 255u, db); }
+        if (!__any(any_a) || !__any(any_b)) continue;
+#pragma unroll
+        for (int ks = 0; ks < 2; ++ks) {
+          i32x8 fa[MI], fb[NI];
+          fragments(buf, ks, fa, fb);
+#pragma unroll
+          for (int j = 0; j < MI; ++j) fa[j] = ka[j] ? fa[j] : (i32x8)0;
+#pragma unroll
+          for (int i = 0; i < NI; ++i) fb[i] = kc[i] ? fb[i] : (i32x8)0;
+          widened(fa, fb, ea, eb);
+          __builtin_amdgcn_sched_barrier(0);     // (or the second half's fragments are read ahead, and registers spill)
+        }
+      }
+      finish();
+    }
   Fp8Out o = p.o;
   if (p.splits > 1) { o.y = (float*)o.y + (int64_t)blockIdx.y * p.M * p.N; o.ldy = p.N; o.type = FT_F32; o.relu = 0; }
   uint8_t* buf = smem8 + wave * 8192;
@@ -714,7 +779,8 @@ __global__ __launch_bounds__(256, 2) void k_fp8_cut(Fp8Cut p) {
 
 // ------------------------------------------------------------------------------------------------------ weight gradients
 // dW = G^T X over the rows of g and x, both cut into blocks of 128 ROWS per column on the way.  The result is fp32 and the sum long, so the
-// 8-bit values go back to bf16 (exactly) for the bf16 matrix instruction.  A block of 8 waves owns 64 NI x 256 results and a range of
+// 8-bit values go back to bf16 for the bf16 matrix instruction, exactly: 16-bit operands have nothing under 2^-133 that rounding could keep (fp16 2^-24),
+// and what would round up to 2^128 takes the value below (tn_max).  A block of 8 waves owns 64 NI x 256 results and a range of
 // 128-row steps.  Per step every wave turns strips of 128 rows x 32 columns round: a lane holds 8 rows x 8 columns (rows rg, rg + 16, ...: a
 // load instruction reads 64 bytes of 16 rows), pairs up its rows (v_perm), the column's maximum crosses the 16 lanes of a DPP row, and each
 // column leaves as 128 bytes of 8-bit values.  Both operands carry the same order of the rows, whatever it is.
@@ -734,17 +800,18 @@ __device__ inline uint32_t pk_max16(uint32_t a, uint32_t b) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
 }
+__device__ inline uint32_t pk_min16(uint32_t a, uint32_t b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
 template <int CTRL> __device__ inline uint32_t dpp_pk_max16(uint32_t v) {
   return pk_max16(v, (uint32_t)__builtin_amdgcn_update_dpp((int)v, (int)v, CTRL, 0xf, 0xf, false));
 }
 
-// one strip: v[i] = eight columns of row i * 16 + rg; tile: [32 columns][128 bytes], scale: their powers of two
-template <int T, int FMT> __device__ inline void tn_quant(u16x8 (&v)[8], uint8_t* tile, float* scale, int lane) {
-  constexpr int EMAX = FMT == F8_E4M3 ? 8 : 15;
+// one strip: v[i] = eight columns of row i * 16 + rg; m: maxima of the eight columns, two to a word.  edge: the least bf16 magnitude that would round up
+// to 2^128 in 8 bits, which the products' bf16 does not hold; it and what lies above become the 8-bit value below, `under`.
+template <int T> __device__ inline void tn_max(u16x8 (&v)[8], uint32_t (&m)[4], uint32_t edge, uint32_t under) {
   constexpr uint32_t INF = T == FT_F16 ? 0x7c00u : 0x7f80u;
-  const int rg = lane & 15, c8 = (lane >> 4) * 8;
-  // maxima of the eight columns, two to a word
-  uint32_t m[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     m[k] = 0;
@@ -756,14 +823,29 @@ template <int T, int FMT> __device__ inline void tn_quant(u16x8 (&v)[8], uint8_t
     m[k] = dpp_pk_max16<0x140>(m[k]);
   }
   const uint32_t most = pk_max16(pk_max16(m[0], m[1]), pk_max16(m[2], m[3]));
-  if (__any((most >> 16) >= INF || (most & 0xffffu) >= INF)) {      // a column with a NaN or an infinity becomes NaN throughout
+  if (T == FT_F16) edge = INF;
+  if (__any((most >> 16) >= edge || (most & 0xffffu) >= edge)) {
+    if constexpr (T == FT_BF16) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
+      for (int i = 0; i < 8; ++i) {
+        i32x4 w = __builtin_bit_cast(i32x4, v[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) w[k] = (int)(pk_min16((uint32_t)w[k] & 0x7fff7fffu, under * 0x10001u) | ((uint32_t)w[k] & 0x80008000u));
+        v[i] = __builtin_bit_cast(u16x8, w);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)        // a column with a NaN or an infinity becomes NaN throughout
       if (((m[j / 2] >> (16 * (j & 1))) & 0xffffu) >= INF) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i][j] = 0x7fff;
       }
   }
+}
+// ... in 8 bits: tile: [32 columns][128 bytes], scale: their powers of two
+template <int T, int FMT> __device__ inline void tn_quant(const u16x8 (&v)[8], const uint32_t (&m)[4], uint8_t* tile, float* scale, int lane) {
+  constexpr int EMAX = FMT == F8_E4M3 ? 8 : 15;
+  const int rg = lane & 15, c8 = (lane >> 4) * 8;
   float s[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
@@ -852,8 +934,11 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
     const int buf = (int)(step - s0) & 1;
     uint8_t* t = smem8 + (buf * COLS + strip * 32) * 128;
     float* sc = scales + buf * COLS + strip * 32;
-    if (FG != F8_E4M3 && strip < TN / 32) tn_quant<T, FG>(v, t, sc, lane);
-    else tn_quant<T, F8_E4M3>(v, t, sc, lane);
+    const bool other = FG != F8_E4M3 && strip < TN / 32;      // (1.9375 2^127 becomes 1.875 2^127 in e4m3, 1.875 2^127 becomes 1.75 2^127 in e5m2)
+    uint32_t m[4];
+    tn_max<T>(v, m, other ? 0x7f70u : 0x7f78u, other ? 0x7f60u : 0x7f70u);
+    if (other) tn_quant<T, FG>(v, m, t, sc, lane);
+    else tn_quant<T, F8_E4M3>(v, m, t, sc, lane);
   };
   const bool busy = n0 + wn * 32 * NI < p.N && k0 + wk * 64 < p.K;      // (waves without results only cut)
   load(s0, wave);

@@ -476,7 +476,8 @@ int aln_fp8_linear(const void* x, int32_t x_type, int64_t ldx, int32_t fmt_x, co
                    int64_t ws_bytes, void* stream);
 
 /* dw [N, K] (fp32, contiguous, overwritten) = G^T X for g [M, N] and x [M, K] as they are (row pitches ldg >= N, ldx >= K, under 2^24), M >= 1: both are cut into
- * blocks of 128 rows per column, g in fmt_g, x in e4m3 -- the weight gradient of y = x W^T.  Bit-reproducible.  ws:
+ * blocks of 128 rows per column, g in fmt_g, x in e4m3 -- the weight gradient of y = x W^T.  Bit-reproducible.  (bf16 magnitudes that would
+ * round up to 2^128 -- from 1.9375 2^127 on in e4m3, 1.875 2^127 in e5m2 -- count as 1.875 2^127 and 1.75 2^127.)  ws:
  * aln_fp8_grad_weight_ws_bytes(same sizes and types) bytes, 16-byte aligned (0: may be NULL). */
 int64_t aln_fp8_grad_weight_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t g_type, int32_t x_type);
 int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, int32_t fmt_g, const void* x, int32_t x_type, int64_t ldx, int64_t M,
