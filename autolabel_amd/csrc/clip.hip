@@ -164,7 +164,7 @@ extern "C" int aln_grad_clip(int32_t n, const void* const* grads, void* const* o
   ALN_REQUIRE(ws && ((uintptr_t)ws & 7) == 0 && ws_bytes >= aln_grad_clip_ws_bytes(n), "grad_clip: the workspace needs %lld bytes, aligned to 8", (long long)aln_grad_clip_ws_bytes(n));
   try {
     std::vector<Span> from, to;
-    from.reserve(n); to.reserve(n);
+    from.reserve(n); to.reserve(n + 3);
     for (int k = 0; k < n; ++k) {
       ALN_REQUIRE(types[k] >= FT_F16 && types[k] <= FT_F32, "grad_clip: tensor %d has the unknown type %d", k, types[k]);
       ALN_REQUIRE(numel[k] >= 0 && numel[k] < (int64_t)1 << 40, "grad_clip: tensor %d has %lld elements", k, (long long)numel[k]);
@@ -178,6 +178,7 @@ extern "C" int aln_grad_clip(int32_t n, const void* const* grads, void* const* o
     }
     if (apply) {    // what is scaled must not be read again by another block of the same launch
       to.insert(to.end(), from.begin(), from.end());
+      for (const void* w : {(const void*)loss_scale, (const void*)norm, (const void*)found_inf}) if (w) to.push_back({(uintptr_t)w, (uintptr_t)w + 4});
       ALN_REQUIRE(!spans_meet(to), "grad_clip: two of the tensors share memory");
     }
   } catch (const std::bad_alloc&) {

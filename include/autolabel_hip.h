@@ -486,7 +486,8 @@ int aln_fp8_grad_weight(const void* g, int32_t g_type, int64_t ldg, int32_t fmt_
 /* ---- global gradient norm and clipping (clip.hip; no counterpart in the reference, whose optimizer step is autolabel/trainer.py:45-48
  * without one).  n tensors of numel[k] elements (host arrays; types[k]: 0 fp16, 1 bf16, 2 fp32; device pointers aligned to their type):
  *   norm = sqrt(sum of all squares, in fp64) / loss_scale;  out[k] = grads[k] * min(1, max_norm / (norm + 1e-6)), rounded to the tensor's type
- * out NULL or out[k] == grads[k]: in place (nothing is written when the factor is 1).  No two tensors may share memory otherwise.
+ * out NULL or out[k] == grads[k]: in place (nothing is written when the factor is 1).  No two tensors may share memory otherwise, nor with
+ * loss_scale, norm and found_inf.
  * apply = 0: the norm only.  loss_scale (device float), norm (device float), found_inf (device word) may be NULL.  A norm that is not finite
  * in fp32 scales nothing and raises *found_inf.  Bit-reproducible.  ws: aln_grad_clip_ws_bytes(n) bytes, 8-byte aligned. */
 int64_t aln_grad_clip_ws_bytes(int32_t n);
