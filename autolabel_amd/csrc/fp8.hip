@@ -17,6 +17,7 @@
 // Layout: q [rows, ldq] bytes, columns [K, 128 ceil(K / 128)) zero; scale [rows, lds] bytes e + 127, lds a multiple of 4, so that the four
 // scales of 512 columns are one aligned 4-byte word.
 #include "common.h"
+#include "fp8_pieces.h"
 #include <type_traits>
 
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -895,26 +896,19 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
     const int C = isg ? p.N : p.K, col = isg ? n0 + strip * 32 : k0 + (strip - TN / 32) * 32;
     if (col >= C) return;                                 // (whole strips behind the last column: cut from what is there, never stored)
     const uint16_t* base = (const uint16_t*)(isg ? p.g : p.x) + step * 128 * ld + col;
-    // Columns stand alone, so what a lane reads behind the last one does not matter as long as it is memory of the tensor: pieces that begin
-    // behind it read the last piece instead, and the last piece's seven values too many lie in the rows behind (ld >= C).
-    const int c = min(c8, (C - 1 - col) & ~7);
-    const int64_t left = p.M - (step + 1) * 128;          // rows behind this step
-    if (!TAIL || (left >= 0 && (col + 32 <= C || left * ld >= 7))) {
+    const int c = tn_column(C, col, c8);
+    if (!TAIL || tn_whole(p.M, ld, C, step, col)) {
       const uint32_t off = 2 * ((uint32_t)rg * (uint32_t)ld + (uint32_t)c);       // bytes
 #pragma unroll
       for (int i = 0; i < 8; ++i) __builtin_memcpy(&v[i], (const uint8_t*)(base + i * 16 * ld) + off, 16);
     } else {
-      // the tensor's end: rows behind the last one read that one and become zero, a piece that would reach over the end begins earlier and
-      // is shifted down (the tensor has eight values or more)
-      const int last = (int)(p.M - 1 - step * 128 < 127 ? p.M - 1 - step * 128 : 127);
-      const int64_t size = (p.M - 1 - step * 128) * ld + C - col;
-      const int end = (int)(size < 0x7fffffff ? size : 0x7fffffff) - 8;            // where the last piece may begin (it may lie before the base)
+      const TnEnd e = tn_end(p.M, ld, C, step, col);
       int over[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const int at = min(rg + 16 * i, last) * (int)ld + c;
-        over[i] = at > end ? at - end : 0;
-        __builtin_memcpy(&v[i], base + (at - over[i]), 16);
+        const TnPiece q = tn_piece(e, (int)ld, rg + 16 * i, c);
+        over[i] = q.over;
+        __builtin_memcpy(&v[i], base + q.at, 16);
       }
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -924,7 +918,7 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
         const int bits = 16 * over[i];
         if (bits >= 64) { w[0] = w[1] >> (bits - 64); w[1] = 0; }
         else if (bits > 0) { w[0] = (w[0] >> bits) | (w[1] << (64 - bits)); w[1] >>= bits; }
-        if (rg + 16 * i > last) w = (u64x2)0;
+        if (rg + 16 * i > e.last) w = (u64x2)0;
         v[i] = __builtin_bit_cast(u16x8, w);
       }
     }
@@ -1273,7 +1267,7 @@ template <int T, int FG, int NI, bool TAIL> static int tn_launch(const Fp8TN& p,
   return 0;
 }
 template <int T, int FG, int NI> static int tn_tail(const Fp8TN& p, hipStream_t st) {
-  return p.M % 128 || p.N % 32 || p.K % 32 ? tn_launch<T, FG, NI, true>(p, st) : tn_launch<T, FG, NI, false>(p, st);
+  return tn_has_tail(p.M, p.N, p.K) ? tn_launch<T, FG, NI, true>(p, st) : tn_launch<T, FG, NI, false>(p, st);
 }
 template <int T> static int tn_pick(const Fp8TN& p, const TnPlan& t, int fmt_g, hipStream_t st) {
   if (fmt_g == F8_E4M3) return t.ni == 4 ? tn_tail<T, F8_E4M3, 4>(p, st) : tn_tail<T, F8_E4M3, 2>(p, st);
