@@ -10,7 +10,6 @@ One launch for the squares and one for the scaling per 120 tensors, whatever the
 import array
 import contextlib
 import math
-import operator
 
 import torch
 
@@ -35,8 +34,7 @@ def _dense(t):
 # Unbound methods mapped over the lists: a list of 60 small gradients costs more on the host than on the device.
 _T = torch.Tensor
 _PLAIN = {torch.Tensor, torch.nn.Parameter}
-_dtype = operator.attrgetter('dtype')
-_requires_grad = operator.attrgetter('requires_grad')
+_dtype, _requires_grad = _T.dtype.__get__, _T.requires_grad.__get__
 
 
 def _check_tracked(name, grads, out, apply):
