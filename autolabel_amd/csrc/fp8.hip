@@ -1142,12 +1142,13 @@ extern "C" int aln_fp8_nt(const void* a, int64_t lda, const uint8_t* sa, int64_t
 static bool lin_fused(int64_t M, int N, int64_t K, int x_type, int y_type, int fmt_w) {
   return (K <= 512 || (K <= 1024 && (N <= 1024 || M <= 512))) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
 }
-// Otherwise k_fp8_cut, where its column tiles are few or there are few rows to cut again: 444219 x 1203 x 40 283 us and 499 in two launches, 65536 x 1280
+// Otherwise k_fp8_cut, where its column tiles are few or there is one row tile to cut again: 444219 x 1203 x 40 283 us and 499 in two launches, 65536 x 1280
 // x 128 40 and 67, 200000 x 1100 x 300 251 and 294, 30000 x 4096 x 384 130 and 136, but x 512 154 and 143; 3 x 1844 x 3304 13.4 and 13.5 (a launch less on the
-// host: 13.4 and 15.4 a call), 300 x 2048 x 2048 19.7 and 21.5, but 1024 x 2048 x 1024 26.6 and 20.5.
+// host: 13.4 and 15.4 a call), 64 x 4096 x 4096 17.8 either way, 128 x 4096 x 4096 20.6 and 22.3, but 129 x 4096 x 4096 23.8 and 21.6, 257 x 4096 x 4096 37.1 and
+// 29.6, 384 x 4096 x 4096 39.9 and 32.6, 384 x 2048 x 4096 28.3 and 19.5 (300 x 2048 x 2048 19.1 and 19.7).
 #define CUT_STEP 1.4                 // us of a lone block's step (nt_plan)
 static bool lin_cut(int64_t M, int N, int x_type, int y_type, int fmt_w) {
-  return (N <= 384 || M <= 384) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
+  return (N <= 384 || M <= 128) && x_type != FT_F32 && y_type != FT_F32 && fmt_w == F8_E4M3;
 }
 static inline int64_t up16(int64_t n) { return (n + 15) / 16 * 16; }
 extern "C" int64_t aln_fp8_linear_ws_bytes(int64_t M, int32_t N, int32_t K, int32_t x_type, int32_t y_type, int32_t fmt_w) {
