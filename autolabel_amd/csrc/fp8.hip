@@ -10,7 +10,8 @@
 // operand: y = sum_b 2^(ex_b + ew_b) sum_{k in b} qx qw costs no instruction beside the matrix instructions.
 // That instruction accumulates in fp32, but aligns the 64 products of a step to the largest of them and drops what lies 13 binades below it
 // (measured; the older v_mfma_f32_32x32x16_fp8_fp8 does the same): 1.3e-5 of the result for Gaussian operands, 7e-5 for values spread over 12
-// binades.  Under the half step of a 16-bit result (4.9e-4, 3.9e-3), far above that of an fp32 one: products with an fp32 result turn the 8-bit
+// binades.  That is under the half step of a 16-bit result (4.9e-4, 3.9e-3) where the sum does not cancel: the half step goes with the sum, what is
+// dropped with its largest term (up to 2^-13 of it a term, K of them).  It is far above the half step of an fp32 result: such products turn the 8-bit
 // values back into bf16, which holds q 2^e exactly but at the ends of the exponents (WIDE_LO), and use the bf16 instruction (5e-8, at half the rate).
 // A block that holds an infinity or a NaN is NaN throughout (its row of the product would be non-finite in every column anyway).
 //
@@ -308,9 +309,9 @@ __device__ inline void store_block(const Fp8Out& o, const f32x16& c0, const f32x
 }
 
 // Blocks b and b + 8 run on the same XCD.  Each XCD takes a run of consecutive work items, so that those that share rows find them in its L2, and
-// all eight have the same number, however few there are: with the row tiles going round the XCDs instead, the one row tile of 64 x 4096 x 4096 was
-// work for 32 of the 256 CUs (40.6 us, so 15.0), and 128 parts of 64 x 512 x 4096 too (18.7, so 5.6).  -1: none left for this block of a grid of
-// xcd_grid(items).
+// all eight have the same number, however few there are.  With the row tiles going round the XCDs instead, one row tile is work for 32 of the 256 CUs: blocks
+// of x and their product for 64 x 4096 x 4096 take 15.0 us this way and 40.6 that way, the 128 parts of 64 x 512 x 4096 5.6 and 18.7.  -1: none left for this
+// block of a grid of xcd_grid(items).
 __device__ inline int xcd_item(int items) {
   const int each = (items + 7) / 8, i = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
   return i < items ? i : -1;
@@ -334,13 +335,14 @@ struct Fp8NT {
 // Two buffers, one barrier per 128 columns: the next step's copies are sent before this one is multiplied.
 // WIDE: the fp32 results' form, 16-bit operands out of the same tiles.
 // Tiles: 256 x 256 by eight waves, or 128 x 128 by four (nt_type), and the contraction in parts where there are few (nt_plan).
-// 8192 x 4096 x 4096 with 16-bit results: 125 .. 134 us by the card's temperature, 2.05 .. 2.2 PFLOP/s (the library's product of unscaled 8-bit
-// values 112); fp32 results 242 us; 256 x 512 x 4096 13 us with the joining of its parts.
+// 8192 x 4096 x 4096 with 16-bit results: 122 .. 134 us by the card's temperature, 2.05 .. 2.25 PFLOP/s (the library's product of unscaled 8-bit
+// values 112); with fp32 results 220 .. 242 us, bound by the bf16 matrix instructions (the library's bf16 product 202; 1345 TFLOP/s at 8192^3 would be 204);
+// 256 x 512 x 4096 13 us with the joining of its parts.
 // What bounds the large ones, in clocks of a CU per 256 x 256 x 128 step: 2050 for the 32 matrix instructions of a SIMD, 170 for the scales, 490 for
 // waves that wait for each other at the barrier, 450 .. 1000 for the 64 KB copied (with the fragments that is 256 KB through LDS, all that 128 bytes
-// a clock give in 2050).  Reading the fragments of a half step ahead across the barrier,
-// copies spread between the matrix instructions (through buffer descriptors, without a branch in the loop), 128 x 128 results a wave with one wave per
-// SIMD, and 4 x 8 groups of tiles per XCD were built and took 144 .. 178 us where this takes 145.
+// a clock give in 2050): the barrier waits for every copy, which has to land inside its own step.  Other schedules, timed in the same runs, in which this one
+// took 145 us (a warm card): the fragments of a half step read ahead across the barrier 144 .. 146, copies spread between the matrix instructions (through
+// buffer descriptors, without a branch in the loop) 148, 128 x 128 results a wave with one wave per SIMD 170 .. 178, 4 x 8 groups of tiles per XCD 145.
 template <int FA, int FB, bool WIDE, int WM, int WN, int MI, int NI>
 __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
   constexpr int BM = WM * MI * 32, BN = WN * NI * 32, NW = WM * WN, ROWS = BM + BN;
@@ -505,7 +507,9 @@ __global__ __launch_bounds__(64 * WM * WN) void k_fp8_nt(Fp8NT p) {
 // flight.  One barrier per tile.
 // Bound by memory where there are many rows: 2^20 x 512 x 512 fp16 479 us, 4.5 TB/s (a large copy reaches 4.6).  50000 rows are four tiles to a block
 // and take 34 us (3.0 TB/s): the first tile's loads and the last one's results have nothing beside them, and tiles of 32 .. 48 rows instead of 64
-// cost more than they hide (36 .. 37.5 us; 2^20 rows 561 .. 634).  4096 rows 10 us, one row 5 us (a launch, and 256 KB of weights).
+// cost more than they hide (36 .. 37.5 us; 2^20 rows 561 .. 634).  4096 rows 10 us (one tile a block: a launch, the block's weights and its rows one
+// after the other, and eight of the sixteen waves only cut), one row 5 us (a launch, and 256 KB of weights over all blocks).  The cut rows go to LDS in
+// 8-byte pieces: a quarter of the kernel's LDS cycles are bank conflicts, 5% of its time.
 // At NKB 4, 7 and 8 the registers do not quite hold everything: 12 .. 84 bytes a lane lie in scratch and are read once per tile.
 struct Fp8Linear {
   const void* x; int64_t ldx;
@@ -786,7 +790,7 @@ __global__ __launch_bounds__(256, 2) void k_fp8_cut(Fp8Cut p) {
 // load instruction reads 64 bytes of 16 rows), pairs up its rows (v_perm), the column's maximum crosses the 16 lanes of a DPP row, and each
 // column leaves as 128 bytes of 8-bit values.  Both operands carry the same order of the rows, whatever it is.
 // Two LDS buffers: while a step is multiplied the strips of the next one are cut into blocks, and the loads of the strip after that are in flight.
-// 2^19 x 512 x 512 fp16: 393 us (0.70 PFLOP/s, and 1.07 GB at 2.7 TB/s).  Every value is read by two blocks (of the same XCD) and cut by both; the
+// 2^19 x 512 x 512 fp16: 393 .. 405 us (0.69 PFLOP/s, and 1.07 GB at 2.7 TB/s), with g in e5m2 the same.  Every value is read by two blocks (of the same XCD) and cut by both; the
 // matrix instructions of a SIMD take 35% of the time, the vector ones that cut and widen most of the rest, and this pattern of loads alone 300 us.
 // Strips of 64 columns by pairs of waves (128-byte pieces of 8 rows, 214 us alone) need a third barrier and took 417 us, two strips on their way per
 // wave 395, sixteen waves or half strips in turn more registers than there are.
@@ -997,7 +1001,7 @@ __global__ __launch_bounds__(512, 2) void k_fp8_tn(Fp8TN p) {
 }
 
 // The slabs of a split contraction, added in a fixed order and rounded once.  Eight threads share four results (their slabs' sums meet through
-// shuffles): with a result's slabs read by one thread alone, 85 slabs of 128 x 512 took 22 us, so 6.8; 64 slabs of 512 x 512 take 15 us, 4.5 TB/s.
+// shuffles): 85 slabs of 128 x 512 6.8 us, and 22 with a result's slabs read by one thread alone; 64 slabs of 512 x 512 15 us, 4.5 TB/s.
 __global__ __launch_bounds__(256) void k_fp8_join(const float* __restrict__ slabs, int splits, int64_t M, int N, Fp8Out o) {
   const int64_t n = M * N;
   for (int64_t q = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> 3; q < (n + 3) / 4; q += (int64_t)gridDim.x * 32) {

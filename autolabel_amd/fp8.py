@@ -159,7 +159,8 @@ def matmul(a, b, out_dtype=torch.float16, relu=False):
 
 def linear(x, weight, relu=False, out_dtype=None, fmt='e4m3', out=None):
     """x [..., K] W^T for ``weight`` = Fp8Blocks of W [N, K] -> [..., N] of x's type (or ``out_dtype``); the rows of x are cut into blocks of
-    ``fmt`` on the way.  ``relu``: negative results become 0.  ``out``: a contiguous tensor of the result's shape to write it into (its type
+    ``fmt`` on the way.  (In a 16-bit result each term may be off by 2^-13 of the
+    largest of its 64; in an fp32 result, at about half the rate, the terms are exact.)  ``relu``: negative results become 0.  ``out``: a contiguous tensor of the result's shape to write it into (its type
     decides the result's); it must not overlap x.  The result carries no gradient: while gradients are tracked, an x that requires one is refused
     (``Linear`` is the layer with its gradients)."""
     if isinstance(x, torch.Tensor) and x.requires_grad and torch.is_grad_enabled():

@@ -399,7 +399,7 @@ class HipPipeline:
     def wide_sem_fwd(self, sout, M, bufs, fp8=False):
         """f = semantic_features([geo, 1]); logits = semantic_out([relu(f), geo, 1]) for M rows of the density head's output.
         bufs: callable name, shape -> fp16 buffer.  Returns (logits [M, Cpad], f [M, D], saved activations).
-        ``fp8`` (inference): the product of semantic_features' last layer in 8-bit blocks (2^20 rows x 512 x 512: 0.50 ms against 0.83; the two layers
+        ``fp8`` (inference): the product of semantic_features' last layer in 8-bit blocks (2^20 rows x 512 x 512: 0.47 ms against 0.76; the two layers
         before it stay with the kernel that generates the first, which 8-bit layers of their own would not beat).  The weight is cut into blocks
         here, at every call (one launch over half a megabyte): a replayed training step changes it without telling anyone."""
         L = self.L
