@@ -61,6 +61,8 @@ def _check(name, grads, out, loss_scale, found_inf, norm):
     for what, w, dt in (('loss_scale', loss_scale, torch.float32), ('found_inf', found_inf, torch.int32), ('norm', norm, torch.float32)):
         if w is not None and (not torch.is_tensor(w) or w.dtype != dt or w.numel() < 1 or w.device != dev):
             raise ValueError(f'{name}: {what} must be a device tensor of {dt} beside the gradients')
+    if norm is not None and norm.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f'{name}: norm requires a gradient, and autograd does not see what is written into it')
     if dev.type != 'cuda':
         raise ValueError(f'{name}: autolabel_amd.clip has no CPU path: needs device tensors')
 
@@ -89,7 +91,8 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf, norm):
         codes = array.array('i', [TYPES[t.dtype] for t in grads])
     dev = grads[0].device
     with contextlib.nullcontext() if dev.index == torch.cuda.current_device() else torch.cuda.device(dev):
-        if norm is None:
+        given = norm is not None
+        if not given:
             norm = torch.empty((), dtype=torch.float32, device=dev)
         ws = torch.empty(H.lib().aln_grad_clip_ws_bytes(n), dtype=torch.uint8, device=dev)
         g, o = array.array('Q', map(_T.data_ptr, grads)), None if out is None else array.array('Q', map(_T.data_ptr, out))
@@ -97,8 +100,11 @@ def _launch(name, grads, max_norm, apply, out, loss_scale, found_inf, norm):
         H.call('aln_grad_clip', n, g.buffer_info()[0], None if o is None else o.buffer_info()[0], sizes.buffer_info()[0], codes.buffer_info()[0], max_norm,
                int(apply), loss_scale.data_ptr() if loss_scale is not None else None, norm.data_ptr(),
                found_inf.data_ptr() if found_inf is not None else None, ws.data_ptr(), ws.numel(), H.raw_stream())
-    if apply:           # (a backward pass that saved one of them notices; inference tensors have no version)
+    # (a backward pass that saved what is written notices; inference tensors have no version)
+    if apply:
         torch.autograd.graph.increment_version(grads if out is None else out)
+    if found_inf is not None or given:
+        torch.autograd.graph.increment_version([w for w in (norm, found_inf) if w is not None])
     return norm
 
 

@@ -34,3 +34,8 @@ def test_without_gradients_a_leaf_is_refused_in_place_only():
         q = p * 2
     with torch.no_grad(), pytest.raises(ValueError, match='no CPU path'):
         clip.clip_grad_norm_([q], 1.0)
+
+
+def test_a_norm_that_requires_a_gradient():
+    with pytest.raises(ValueError, match='norm requires a gradient'):
+        clip.grad_norm([torch.zeros(3)], norm=torch.zeros((), requires_grad=True))

@@ -76,3 +76,17 @@ def test_inference_tensors(clip):
     clip.clip_grad_norm_([t], 0.5, out=[o])
     clip.clip_grad_norm_([t], 0.5)
     assert abs(float(clip.grad_norm([t])) - 0.5) < 1e-5 and abs(float(clip.grad_norm([o])) - 0.5) < 1e-5
+
+
+def test_the_norm_and_the_flag_are_written_too(clip):
+    t = torch.ones(100, device='cuda')
+    leaf = torch.ones((), device='cuda', requires_grad=True)
+    for apply in (False, True):
+        norm, flag = torch.ones((), device='cuda'), torch.zeros(1, dtype=torch.int32, device='cuda')
+        loss, version = leaf * norm, flag._version
+        clip.clip_grad_norm_([t], 1.0, norm=norm, found_inf=flag) if apply else clip.grad_norm([t], norm=norm, found_inf=flag)
+        assert flag._version > version
+        with pytest.raises(RuntimeError, match='modified by an inplace operation'):
+            loss.backward()
+    with pytest.raises(ValueError, match='norm requires a gradient'):
+        clip.grad_norm([t], norm=torch.zeros((), device='cuda', requires_grad=True))
